@@ -219,6 +219,11 @@ def work(case):
 
 
 # ---- the definition in 64 bits ---------------------------------------------------------------------------------------------
+def _power(e):
+    """2^e in 64 bits, exactly (e from -1022 on)."""
+    return ((e.to(torch.int64) + 1023) << 52).view(torch.float64)
+
+
 def _exact_blocks(v):
     """Codes (as numbers) and exponents of rows given in 64 bits, padded to whole blocks."""
     M, K = v.shape
@@ -230,21 +235,21 @@ def _exact_blocks(v):
     mantissa, power = torch.frexp(top)                       # top = mantissa 2^power, 448 = 0.875 2^9
     e = torch.where(mantissa <= 0.875, power - 9, power - 8)
     e = torch.where(top > 0, e, torch.full_like(e, -126)).clamp(-126, 120)
-    scaled = torch.ldexp(whole, -e[..., None])
+    scaled = whole * _power(-e)[..., None]
     _, p = torch.frexp(scaled)
-    step = torch.ldexp(torch.ones_like(scaled), torch.clamp(p - 1, min=-6) - 3)       # four bits of a value, steps of 2^-9 at least
+    step = _power(torch.clamp(p - 1, min=-6) - 3)       # four bits of a value, steps of 2^-9 at least
     return torch.round(scaled / step) * step, e
 
 
 def _exact_rows(v):
     codes, e = _exact_blocks(v)
-    return torch.ldexp(codes, e[..., None]).reshape(v.shape[0], -1)[:, :v.shape[1]]
+    return (codes * _power(e)[..., None]).reshape(v.shape[0], -1)[:, :v.shape[1]]
 
 
 def _exact_weight(w):
     codes, scales = w
     e = (scales.to(torch.int32) - 127).unsqueeze(-1).expand(*scales.shape, BLOCK).reshape(scales.shape[0], -1)[:, :codes.shape[1]]
-    return torch.ldexp(codes.to(torch.float64), e)
+    return codes.to(torch.float64) * _power(e)
 
 
 def _exact_unit(name, g, u):
