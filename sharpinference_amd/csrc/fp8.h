@@ -1,0 +1,116 @@
+// Rows and weights in 8-bit floating point: e4m3 codes, and one power of two for every 128 values of a row.
+//
+// Format.  A row is cut into blocks of 128 values (the last one filled up with zeros).  A block's byte s, from 1 to 247, stands for the
+// scale 2^(s - 127): the smallest with which the block's largest finite magnitude is at most 448, e4m3's largest value.  A value v is
+// stored as e4m3(v 2^(127 - s)), to nearest, ties to even.  Both the byte and the scaled value come from exact arithmetic (an exponent
+// read from the bits, a product by a power of two), so every kernel that quantises a row gives the same codes.  Infinities and NaN
+// become e4m3's NaN and do not count for the scale.
+//
+// Why powers of two: v_mfma_scale_f32_*_f8f6f4 multiplies each operand row by such a byte (E8M0) itself, for every 32 of k.  The scales of a
+// block of 128 then cost no instruction of their own and the sums stay in the accumulators; a scale of full precision would take a
+// multiply-add per accumulator and block, and gains nothing where the values are floating point themselves.
+//
+// Accuracy of that instruction, measured: of eight products on end those some 2^-13 below the largest are cut, the groups of eight
+// are added in float: 1.5e-5 of the result's rms for normal values.  Results are therefore offered as bfloat16 only.
+//
+// Layouts.  Rows [M]: codes row by row, 128 U bytes each (U blocks), bytes of scales row by row, 4 U4 each (U4 = U / 4 rounded up).
+// Weights [N, K]: rows in tiles of 32 (filled up with zeros), tile by tile and block by block, 4 KB each in the order
+// [half s of 64 k][piece p][group g][row r of 32][16 bytes], k = 64 s + 32 g + 16 p + byte: a wave's 16-byte loads of v_mfma 32x32x64's
+// operand are one kilobyte on end, and those of 16x16x128 four runs of 256.  Their scales [tile][U4][row of 32][4 blocks].
+#pragma once
+#include "common.h"
+
+typedef __attribute__((ext_vector_type(8))) int i32x8;
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
+
+constexpr int kF8Block = 128;                 // values that share a scale
+constexpr int kF8Tile = 32;                   // weight rows of a tile
+constexpr int kF8TileBytes = kF8Tile * kF8Block;
+constexpr uint32_t kF8Nan = 0x7f;
+
+static inline __host__ __device__ int f8_blocks(int k) { return (k + kF8Block - 1) / kF8Block; }
+static inline __host__ __device__ int f8_scale_stride(int k) { return (f8_blocks(k) + 3) & ~3; }     // bytes of a row's scales
+static inline __host__ __device__ int f8_padded_rows(int n) { return (n + kF8Tile - 1) / kF8Tile * kF8Tile; }
+// bytes of a stored matrix's scales (codes: padded rows x blocks x 128)
+static inline __host__ __device__ size_t f8_scale_bytes(int padded_rows, int k) { return (size_t)padded_rows * f8_scale_stride(k); }
+
+// The block's byte from the bits of its largest finite magnitude (448 = 1.75 x 2^8).
+__device__ __forceinline__ int f8_scale_of(uint32_t top_bits) {
+  const int s = (int)(top_bits >> 23) - 8 + ((top_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return s < 1 ? 1 : s;
+}
+__device__ __forceinline__ float f8_scale_value(int s) { return __uint_as_float((uint32_t)s << 23); }
+
+typedef __attribute__((ext_vector_type(2))) short s16x2_t;
+typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2v_t;
+// Four values' codes, of floats or of two pairs of bfloat16, divided by `scale` (a power of two).
+__device__ __forceinline__ uint32_t f8_codes4(float a, float b, float c, float d, float scale) {
+  s16x2_t v = {0, 0};
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(v, a, b, scale, false);
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(v, c, d, scale, true);
+  return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ uint32_t f8_codes4(uint32_t lo, uint32_t hi, float scale) {
+  s16x2_t v = {0, 0};
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(v, __builtin_bit_cast(bf16x2v_t, lo), scale, false);
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(v, __builtin_bit_cast(bf16x2v_t, hi), scale, true);
+  return __builtin_bit_cast(uint32_t, v);
+}
+struct MaxBits {    // the larger of two magnitudes by their bits (NaN is the largest, not lost)
+  __device__ __forceinline__ float operator()(float a, float b) const {
+    const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+    return __uint_as_float(x > y ? x : y);
+  }
+};
+
+// 32 neighbouring values of one row as they lie in memory, in lanes (row r of 16, quarter g of the block of 128): what the 16x16x128
+// instruction takes as an operand once they are codes.  f8_codes gives the codes and the block's byte; the four lanes of a row meet.
+template <typename T> struct F8Raw;
+template <> struct F8Raw<bf16_t> {
+  static constexpr int kLoads = 4, kEach = 8;
+  u32x4_t v[4];
+  __device__ __forceinline__ uint32_t top() const {
+    u16x2_t m = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, v[i / 4][i % 4] & 0x7fff7fffu));
+    return (uint32_t)(m[0] > m[1] ? m[0] : m[1]) << 16;
+  }
+  __device__ __forceinline__ uint32_t top_of_finite() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t lo = v[i / 4][i % 4] & 0x7fffu, hi = v[i / 4][i % 4] >> 16 & 0x7fffu;
+      m = lo < 0x7f80u && lo > m ? lo : m;
+      m = hi < 0x7f80u && hi > m ? hi : m;
+    }
+    return m << 16;
+  }
+  __device__ __forceinline__ void nan_for_infinity() {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      uint32_t d = v[i / 4][i % 4];
+      if ((d & 0x7f80u) == 0x7f80u) d |= 0x7fffu;
+      if ((d & 0x7f800000u) == 0x7f800000u) d |= 0x7fff0000u;
+      v[i / 4][i % 4] = d;
+    }
+  }
+  __device__ __forceinline__ uint32_t codes(int i, float scale) const { return f8_codes4(v[i / 2][i % 2 * 2], v[i / 2][i % 2 * 2 + 1], scale); }
+};
+template <typename T> __device__ __forceinline__ i32x8 f8_codes(F8Raw<T>& raw, int& s) {
+  auto meet = [](uint32_t top) { return __float_as_uint(reduce16(reduce32(__uint_as_float(top), MaxBits{}), MaxBits{})); };
+  uint32_t top = meet(raw.top());
+  if (__builtin_amdgcn_ballot_w64(top >= 0x7f800000u)) {      // some value of the wave is not finite
+    top = meet(raw.top_of_finite());
+    raw.nan_for_infinity();
+  }
+  s = f8_scale_of(top);
+  const float scale = f8_scale_value(s);
+  i32x8 c;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i] = (int)raw.codes(i, scale);
+  return c;
+}

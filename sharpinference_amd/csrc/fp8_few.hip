@@ -1,0 +1,589 @@
+// Products of few rows with weights in 8-bit floating point (fp8.h holds the format), weight-streaming: every block reads its tiles of the
+// matrix once, with the streaming hint, and everything else is arranged around that.  Three forms:
+//   plain   out[M, N] = q(x) W^T, bfloat16
+//   gated   h = act(s g) (s u) with (g | u) = q(x) W^T, rounded to bfloat16: the first half of a feed-forward, for one matrix or for the
+//           experts that a router picked (a block finds the rows of its expert among the picks itself)
+//   sum     out[t] = sum_j w[t, j] q(h[t, j]) W_e^T over the token's picks e (and an always-on expert): the second half, with the sum
+// q(.): rows are quantised where they are read, by the lanes that need them (32 values a lane, four lanes a block of 128): no launch and
+// no pass of its own; or they come as codes already.
+//
+// Bound: bytes of the weights.  Each wave takes blocks of 128 of k in turn, one 4 KB unit of a tile of 32 weight rows (or half of it)
+// at a time through v_mfma_scale_f32_16x16x128: W is the A operand (rows = n), x the B operand (up to 16 rows a row block).  A lane ends
+// up with four neighbouring n of one x row; the waves' sums meet in LDS and are added in wave order.
+//
+// The sum form deals all blocks of k of all experts that occur to S blocks a tile in equal shares, whatever the picks: a column tile has few
+// blocks (160 of 32 columns at 5,120), the experts many bytes.  A column of the product is a token, whose row of h is looked up for each
+// expert, so that all experts add up in the same accumulators.  Their partial sums go through memory; the last block of a tile to
+// finish adds them in the order of the shares: the result does not depend on which that is.
+#include "fp8.h"
+
+namespace {
+
+constexpr int FW = 8;                  // waves a block
+constexpr int kFewRows = 64;           // rows (tokens) of a call at most: four row blocks
+constexpr int kFewPairs = 1024;        // (token, pick) pairs of a call at most
+constexpr int kFewExperts = 1024;
+constexpr int kRound = 2;              // (tile, row block) pairs that meet in LDS at a time
+
+struct F8Matrix {
+  const uint8_t* codes;    // [matrices][rows / 32][U][4096]
+  const uint8_t* scales;   // [matrices][rows / 32][U4][32][4]
+  int rows, U;             // rows of one matrix (a multiple of 32), blocks of 128 of k
+};
+
+// the picks of a call (ids null: one matrix, row = token)
+struct F8Picks {
+  const int* ids;          // [T, k]
+  const float* w;          // [T, k] or null
+  int T, k, E;
+  int shared;              // one more matrix (number E) that every token goes through: rows T k + t
+};
+
+// A wave's view of one 16-row half tile of a matrix.
+struct F8Lane {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  __device__ __forceinline__ void at(const F8Matrix& w, size_t matrix, int half_tile, int r, int g) {
+    const int last = w.rows / 16 - 1, t = half_tile < last ? half_tile : last;      // (beyond the last: read, never stored)
+    const size_t tile = matrix * (w.rows / 32) + (t >> 1);
+    codes = w.codes + tile * w.U * kF8TileBytes + (g >> 1) * 2048 + (g & 1) * 512 + (t & 1) * 256 + r * 16;
+    scales = w.scales + tile * ((w.U + 3) >> 2) * 128 + ((t & 1) * 16 + r) * 4;
+  }
+  __device__ __forceinline__ i32x8 load(int u, int& s) const {
+    const i32x4 a = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(codes + (size_t)u * kF8TileBytes));
+    const i32x4 b = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(codes + (size_t)u * kF8TileBytes + 1024));
+    s = scales[(u >> 2) * 128 + (u & 3)];
+    return i32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  }
+};
+
+// A lane's 32 values of an x row for block u of k, before they are codes.
+struct F8Codes {};
+template <typename XT> struct F8Row {
+  F8Raw<XT> raw;
+  __device__ __forceinline__ void load(const void* x, const uint8_t*, size_t row, int K, int u, int g) {
+    const XT* p = (const XT*)x + row * K;
+#pragma unroll
+    for (int i = 0; i < F8Raw<XT>::kLoads; ++i) {
+      const int k = u * kF8Block + g * 32 + i * F8Raw<XT>::kEach;
+      raw.v[i] = *reinterpret_cast<const u32x4_t*>(p + min(k, K - F8Raw<XT>::kEach));
+    }
+  }
+  __device__ __forceinline__ i32x8 codes(int K, int u, int g, int& s) {
+    if (u * kF8Block + kF8Block > K) {                  // the last block of a row that ends inside of it (the same for the wave)
+#pragma unroll
+      for (int i = 0; i < F8Raw<XT>::kLoads; ++i)
+        if (u * kF8Block + g * 32 + i * F8Raw<XT>::kEach >= K) raw.v[i] = u32x4_t{0, 0, 0, 0};
+    }
+    return f8_codes(raw, s);
+  }
+};
+template <> struct F8Row<F8Codes> {
+  i32x4 a, b;
+  int byte;
+  __device__ __forceinline__ void load(const void* x, const uint8_t* scales, size_t row, int K, int u, int g) {
+    const uint8_t* p = (const uint8_t*)x + (row * f8_blocks(K) + u) * kF8Block + g * 32;
+    a = *reinterpret_cast<const i32x4*>(p);
+    b = *reinterpret_cast<const i32x4*>(p + 16);
+    byte = scales[row * f8_scale_stride(K) + u];
+  }
+  __device__ __forceinline__ i32x8 codes(int, int, int, int& s) {
+    s = byte;
+    return i32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  }
+};
+
+__device__ __forceinline__ f32x4 f8_product(const i32x8& w, const i32x8& x, const f32x4& c, int ws, int xs) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 0, 0, 0, ws, 0, xs);
+}
+
+// Four neighbouring columns from n on of one row of `columns`.
+__device__ __forceinline__ void store_columns(bf16_t* row, int n, int columns, const f32x4& v) {
+  if (n + 4 <= columns && ((uintptr_t)(row + n) & 7) == 0) {
+    *reinterpret_cast<uint2*>(row + n) = make_uint2(f32_to_bf16_pair(v[0], v[1]), f32_to_bf16_pair(v[2], v[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < columns) row[n + i] = f32_to_bf16(v[i]);
+  }
+}
+
+// plain and gated.  R half tiles a block: of distinct columns (plain), or R / 2 of gate columns and the up columns beside them (gated).
+// n_out: columns of the result that exist; stride: of a stored row (gated: the columns from n_out to it are zeros, as their weights are).
+template <int R, int MB, typename XT, bool GATED>
+__global__ __launch_bounds__(FW* kWave, 4) void fp8_few_kernel(const void* __restrict__ x, const uint8_t* __restrict__ x_scales, F8Matrix W,
+                                                               bf16_t* __restrict__ out, int n_out, int stride, int M, int K, GatedAct act,
+                                                               F8Picks pk, int* __restrict__ clear, int n_clear) {
+  constexpr int TG = GATED ? R / 2 : R;
+  constexpr int RT = GATED ? R : kRound;
+  __shared__ f32x4 red[FW][RT][kWave];
+  __shared__ short members[GATED ? kFewPairs + kFewRows : 1];
+  __shared__ int flags[GATED ? kFewExperts : 1];
+  __shared__ int n_members;
+  const int lane = threadIdx.x & (kWave - 1), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  int rows = M, expert = 0;
+  const bool picked = GATED && pk.ids != nullptr;
+  if constexpr (GATED) {
+    if (clear && blockIdx.x == 0 && blockIdx.y == 0)          // the counters of the sum behind this launch
+      for (int i = threadIdx.x; i < n_clear; i += FW * kWave) clear[i] = 0;
+  }
+  if (picked) {
+    // Group 0 is the always-on matrix, if there is one; the others are experts, all of them where there are as many groups, else the
+    // distinct ones among the picks in their order (the groups that find none are the grid's last blocks).
+    const int n_pairs = pk.T * pk.k, group = (int)blockIdx.y - pk.shared;
+    if (group < 0) {
+      expert = pk.E;
+      rows = pk.T;
+    } else {
+      if ((int)gridDim.y - pk.shared == pk.E) {
+        expert = group;
+      } else {
+        int mine[kFewPairs / (FW * kWave)];
+#pragma unroll
+        for (int i = 0; i < kFewPairs / (FW * kWave); ++i) {
+          const int p = i * FW * kWave + threadIdx.x;
+          mine[i] = p < n_pairs ? pk.ids[p] : -1;
+        }
+        for (int i = threadIdx.x; i < pk.E; i += FW * kWave) flags[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kFewPairs / (FW * kWave); ++i)
+          if ((unsigned)mine[i] < (unsigned)pk.E) flags[mine[i]] = 1;
+        __syncthreads();
+        int before = 0;
+        expert = -1;
+        for (int c = 0; c < pk.E && expert < 0; c += kWave) {
+          unsigned long long m = __builtin_amdgcn_ballot_w64(c + lane < pk.E && flags[c + lane] != 0);
+          const int n = __popcll(m);
+          if (group < before + n) {
+            for (int i = before; i < group; ++i) m &= m - 1;
+            expert = c + __ffsll((long long)m) - 1;
+          }
+          before += n;
+        }
+      }
+      if (expert < 0) return;                   // (the same for the block)
+      if (w == 0) {
+        int n = 0;
+        for (int c = 0; c < n_pairs; c += kWave) {
+          const bool mine = c + lane < n_pairs && pk.ids[c + lane] == expert;
+          const unsigned long long m = __builtin_amdgcn_ballot_w64(mine);
+          if (mine) members[n + __popcll(m & ((1ull << lane) - 1ull))] = (short)(c + lane);
+          n += __popcll(m);
+        }
+        if (lane == 0) n_members = n;
+      }
+      __syncthreads();
+      rows = n_members;
+    }
+  }
+  if (rows <= 0) return;
+  const bool routed = picked && expert < pk.E;
+  auto out_row = [&](int m) { return routed ? (int)members[m] : picked ? pk.T * pk.k + m : m; };
+  auto x_row = [&](int m) { return routed ? members[m] / pk.k : m; };
+  const int n_base = blockIdx.x * 16 * TG;
+  F8Lane wl[R];
+#pragma unroll
+  for (int t = 0; t < R; ++t)
+    wl[t].at(W, expert, n_base / 16 + t % TG + (GATED && t >= TG ? W.rows / 32 : 0), r, g);
+  // (of a gated matrix the up rows begin at half its rows, a multiple of 32: half tile rows / 32)
+
+  for (int rb = 0; rb * 16 < rows; rb += MB) {
+    size_t xr[MB];
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) xr[mb] = x_row(min((rb + mb) * 16 + r, rows - 1));
+    f32x4 acc[R][MB];
+#pragma unroll
+    for (int t = 0; t < R; ++t)
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) acc[t][mb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    struct Unit {
+      i32x8 wf[R];
+      int ws[R];
+      F8Row<XT> xf[MB];
+    };
+    auto load_unit = [&](int u, Unit& un) {
+#pragma unroll
+      for (int t = 0; t < R; ++t) un.wf[t] = wl[t].load(u, un.ws[t]);
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        if (mb > 0 && (rb + mb) * 16 >= rows) continue;       // (the same for the block)
+        un.xf[mb].load(x, x_scales, xr[mb], K, u, g);
+      }
+    };
+    auto use_unit = [&](int u, Unit& un) {
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        if (mb > 0 && (rb + mb) * 16 >= rows) continue;
+        int xs;
+        const i32x8 c = un.xf[mb].codes(K, u, g, xs);
+#pragma unroll
+        for (int t = 0; t < R; ++t) acc[t][mb] = f8_product(un.wf[t], c, acc[t][mb], un.ws[t], xs);
+      }
+    };
+    if constexpr (MB == 1) {
+      Unit a, b;
+      int u = w;
+      if (u < W.U) load_unit(u, a);
+      for (; u + 2 * FW < W.U; u += 2 * FW) {
+        load_unit(u + FW, b);
+        use_unit(u, a);
+        load_unit(u + 2 * FW, a);
+        use_unit(u + FW, b);
+      }
+      if (u + FW < W.U) {
+        load_unit(u + FW, b);
+        use_unit(u, a);
+        use_unit(u + FW, b);
+      } else if (u < W.U) {
+        use_unit(u, a);
+      }
+    } else {
+      for (int u = w; u < W.U; u += FW) {
+        Unit a;
+        load_unit(u, a);
+        use_unit(u, a);
+      }
+    }
+
+    if constexpr (GATED) {
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        if (mb > 0 && (rb + mb) * 16 >= rows) continue;
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < R; ++t) red[w][t][lane] = acc[t][mb];
+        __syncthreads();
+        if (w < TG) {
+          f32x4 gv = red[0][w][lane], uv = red[0][w + TG][lane];
+#pragma unroll
+          for (int ww = 1; ww < FW; ++ww) {
+            gv += red[ww][w][lane];
+            uv += red[ww][w + TG][lane];
+          }
+          const int m = (rb + mb) * 16 + r, n = n_base + w * 16 + g * 4;
+          if (m < rows && n < stride) {
+            const int orow = out_row(m);
+            const bool scaled = routed && pk.w != nullptr;
+            const float sc = scaled ? pk.w[orow] : 1.0f;
+            f32x4 o;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = gated_f32(act, gv[i], uv[i], sc, scaled);
+            store_columns(out + (size_t)orow * stride, n, stride, o);
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int p0 = 0; p0 < R * MB; p0 += kRound) {
+        bool any = false;
+#pragma unroll
+        for (int p = 0; p < kRound; ++p) any = any || (p0 + p < R * MB && (rb + (p0 + p) % MB) * 16 < rows);
+        if (!any) continue;
+        __syncthreads();
+#pragma unroll
+        for (int p = 0; p < kRound; ++p)
+          if (p0 + p < R * MB) red[w][p][lane] = acc[(p0 + p) / MB][(p0 + p) % MB];
+        __syncthreads();
+        if (w < kRound && p0 + w < R * MB) {
+          const int t = (p0 + w) / MB, mb = (p0 + w) % MB;
+          f32x4 v = red[0][w][lane];
+#pragma unroll
+          for (int ww = 1; ww < FW; ++ww) v += red[ww][w][lane];
+          const int m = (rb + mb) * 16 + r, n = n_base + t * 16 + g * 4;
+          if (m < rows && n < n_out) store_columns(out + (size_t)m * stride, n, n_out, v);
+        }
+      }
+    }
+  }
+}
+
+// The sum over a token's picks.  R half tiles of columns a block, MB row blocks of tokens; blockIdx.y: the share of the blocks of k.
+// part [S][tiles][MB][R][64 lanes] float4, counters [tiles] zero before the launch (both unused if S is 1).
+template <int R, int MB, typename XT>
+__global__ __launch_bounds__(FW* kWave, 4) void fp8_sum_kernel(const void* __restrict__ h, const uint8_t* __restrict__ h_scales, F8Matrix W,
+                                                               bf16_t* __restrict__ out, int n_out, int K, F8Picks pk, int weighted,
+                                                               f32x4* __restrict__ part, int* __restrict__ counters) {
+  __shared__ f32x4 red[FW][kRound][kWave];
+  __shared__ int ids[kFewPairs];
+  __shared__ float wts[kFewPairs];
+  __shared__ int occurs[kFewExperts];           // times that one token picks the expert, at most
+  __shared__ int entry[kFewPairs + 1];          // expert | occurrence << 16
+  __shared__ int n_entries, is_last;
+  const int lane = threadIdx.x & (kWave - 1), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const int n_pairs = pk.ids ? pk.T * pk.k : 0;
+  if (pk.ids) {
+    for (int i = threadIdx.x; i < n_pairs; i += FW * kWave) {
+      ids[i] = pk.ids[i];
+      if (weighted) wts[i] = pk.w[i];
+    }
+    for (int i = threadIdx.x; i < pk.E; i += FW * kWave) occurs[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n_pairs; i += FW * kWave) {
+      const int e = ids[i];
+      int n = 1;
+      for (int j = i / pk.k * pk.k; j < i; ++j) n += ids[j] == e;
+      if ((unsigned)e < (unsigned)pk.E) atomicMax(&occurs[e], n);
+    }
+    __syncthreads();
+    if (w == 0) {                               // (expert, occurrence) entries in the experts' order, the always-on one last
+      int n = 0;
+      for (int c = 0; c < pk.E; c += kWave) {
+        const int mine = c + lane < pk.E ? occurs[c + lane] : 0;
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) {
+          const int up = __shfl_up(upto, o, kWave);
+          if (lane >= o) upto += up;
+        }
+        for (int i = 0; i < mine; ++i) entry[n + upto - mine + i] = (c + lane) | i << 16;
+        n += __shfl(upto, kWave - 1, kWave);
+      }
+      if (pk.shared && lane == 0) entry[n] = pk.E;
+      if (lane == 0) n_entries = n + pk.shared;
+    }
+    __syncthreads();
+  }
+  const int entries = pk.ids ? __builtin_amdgcn_readfirstlane(n_entries) : 1;
+  const int S = gridDim.y, share = blockIdx.y, all = entries * W.U;      // (entries x blocks of k: below 2^31, checked on the host)
+  const int first = (int)((long long)all * share / S), end = (int)((long long)all * (share + 1) / S);
+  const int n_base = blockIdx.x * 16 * R;
+
+  f32x4 total[R][MB];
+#pragma unroll
+  for (int t = 0; t < R; ++t)
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) total[t][mb] = f32x4{0.f, 0.f, 0.f, 0.f};
+  struct Unit {
+    i32x8 wf[R];
+    int ws[R], u;
+    F8Row<XT> xf[MB];
+    float weight[MB];
+    int row[MB];
+  };
+  auto load_unit = [&](int i, Unit& un) {
+    const int at = i / W.U;
+    un.u = i - at * W.U;
+    const int code = pk.ids ? __builtin_amdgcn_readfirstlane(entry[at]) : 0;
+    const int e = code & 0xffff, occurrence = code >> 16;
+#pragma unroll
+    for (int t = 0; t < R; ++t) {
+      F8Lane wl;
+      wl.at(W, e, n_base / 16 + t, r, g);
+      un.wf[t] = wl.load(un.u, un.ws[t]);
+    }
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      const int tok = mb * 16 + r;
+      int row = -1;
+      float weight = 1.f;
+      if (tok < pk.T) {
+        if (!pk.ids) row = tok;
+        else if (e == pk.E) row = n_pairs + tok;
+        else {
+          int seen = 0;
+          for (int j = 0; j < pk.k; ++j) {
+            const int p = tok * pk.k + j;
+            if (ids[p] == e) {
+              if (seen == occurrence) {
+                row = p;
+                if (weighted) weight = wts[p];
+              }
+              ++seen;
+            }
+          }
+        }
+      }
+      un.row[mb] = row;
+      un.weight[mb] = weight;
+      un.xf[mb].load(h, h_scales, row < 0 ? 0 : row, K, un.u, g);      // (row 0: read for a token without this expert, never added)
+    }
+  };
+  auto use_unit = [&](Unit& un) {
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      int xs;
+      const i32x8 c = un.xf[mb].codes(K, un.u, g, xs);
+#pragma unroll
+      for (int t = 0; t < R; ++t) {
+        const f32x4 v = f8_product(un.wf[t], c, f32x4{0.f, 0.f, 0.f, 0.f}, un.ws[t], xs);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) total[t][mb][i] = un.row[mb] >= 0 ? fmaf(un.weight[mb], v[i], total[t][mb][i]) : total[t][mb][i];
+      }
+    }
+  };
+  if constexpr (MB == 1) {
+    Unit a, b;
+    int i = first + w;
+    if (i < end) load_unit(i, a);
+    for (; i + 2 * FW < end; i += 2 * FW) {
+      load_unit(i + FW, b);
+      use_unit(a);
+      load_unit(i + 2 * FW, a);
+      use_unit(b);
+    }
+    if (i + FW < end) {
+      load_unit(i + FW, b);
+      use_unit(a);
+      use_unit(b);
+    } else if (i < end) {
+      use_unit(a);
+    }
+  } else {
+    for (int i = first + w; i < end; i += FW) {
+      Unit a;
+      load_unit(i, a);
+      use_unit(a);
+    }
+  }
+
+  auto store = [&](int t, int mb, const f32x4& v) {
+    const int tok = mb * 16 + r, n = n_base + t * 16 + g * 4;
+    if (tok < pk.T && n < n_out) store_columns(out + (size_t)tok * n_out, n, n_out, v);
+  };
+  // part: [share][tile][pair p][lane]
+  const size_t tile_parts = (size_t)R * MB * kWave, share_parts = (size_t)gridDim.x * tile_parts;
+#pragma unroll
+  for (int p0 = 0; p0 < R * MB; p0 += kRound) {
+    __syncthreads();
+#pragma unroll
+    for (int p = 0; p < kRound; ++p)
+      if (p0 + p < R * MB) red[w][p][lane] = total[(p0 + p) / MB][(p0 + p) % MB];
+    __syncthreads();
+    if (w < kRound && p0 + w < R * MB) {
+      f32x4 v = red[0][w][lane];
+#pragma unroll
+      for (int ww = 1; ww < FW; ++ww) v += red[ww][w][lane];
+      if (S == 1) store((p0 + w) / MB, (p0 + w) % MB, v);
+      else part[share * share_parts + blockIdx.x * tile_parts + (size_t)(p0 + w) * kWave + lane] = v;
+    }
+  }
+  if (S == 1) return;
+  // what the block wrote is everyone's before its ticket counts; who draws the last ticket adds the shares up in their order
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int before = __hip_atomic_fetch_add(&counters[blockIdx.x], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    is_last = before == S - 1;
+  }
+  __syncthreads();
+  if (!is_last) return;
+  __threadfence();
+  for (int p = w; p < R * MB; p += FW) {
+    const float* src = reinterpret_cast<const float*>(part + blockIdx.x * tile_parts + (size_t)p * kWave + lane);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += __hip_atomic_load(src + s * share_parts * 4 + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    store(p / MB, p % MB, v);
+  }
+}
+
+// x operand of a call: codes, or (up to 16 rows) bfloat16 whose runs of eight lie at 16-byte addresses
+enum : int { X_BF16 = DT_BF16, X_CODES = 2 };
+bool rows_ok(const void* x, int kind, int M, int K) {
+  if (((uintptr_t)x & 15) != 0) return false;
+  return kind == X_CODES || (kind == X_BF16 && K % 8 == 0 && M <= 16);
+}
+bool matrix_ok(const F8Matrix& W, long long matrices) {
+  return W.rows > 0 && W.rows % kF8Tile == 0 && W.U > 0 && matrices > 0 && (long long)W.rows * W.U < 0x7fffffffLL;
+}
+
+}  // namespace
+
+// out [M, N] bfloat16 = q(x [M, K]) W^T, M <= 64.  kind: X_*; w_rows: stored rows of W (N up to a multiple of 32); R 1 or 2 half tiles a block.
+SHARPI_EXPORT int sharpi_fp8_few(const void* x, const void* x_scales, int kind, const void* w_codes, const void* w_scales, int w_rows, void* out,
+                                 int M, int N, int K, int R, hipStream_t stream) {
+  if (M <= 0) return SHARPI_OK;
+  const F8Matrix W{(const uint8_t*)w_codes, (const uint8_t*)w_scales, w_rows, f8_blocks(K)};
+  if (M > kFewRows || N <= 0 || K <= 0 || w_rows != f8_padded_rows(N) || !matrix_ok(W, 1) || !rows_ok(x, kind, M, K)) return SHARPI_ERR_ARG;
+  const int mb = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+  const dim3 grid((unsigned)ceil_div(N, 16 * R)), block(FW * kWave);
+#define FF(RV, MBV, XT) \
+  fp8_few_kernel<RV, MBV, XT, false><<<grid, block, 0, stream>>>(x, (const uint8_t*)x_scales, W, (bf16_t*)out, N, N, M, K, GatedAct{}, F8Picks{}, nullptr, 0)
+#define FF_MB(RV, XT)        \
+  if (mb == 1) FF(RV, 1, XT); \
+  else if (mb == 2) FF(RV, 2, XT); \
+  else FF(RV, 4, XT)
+#define FF_X(RV)                                          \
+  if (kind == X_CODES) { FF_MB(RV, F8Codes); }            \
+  else if (mb == 1) FF(RV, 1, bf16_t);                    \
+  else return SHARPI_ERR_ARG
+  if (R == 1) { FF_X(1); }
+  else if (R == 2) { FF_X(2); }
+  else return SHARPI_ERR_ARG;
+#undef FF_X
+#undef FF_MB
+#undef FF
+  SHARPI_CHECK_LAUNCH();
+  return SHARPI_OK;
+}
+
+static bool picks_ok(const F8Picks& p) {
+  if (p.T <= 0 || p.T > kFewRows || p.E <= 0 || p.E > kFewExperts) return false;
+  if (!p.ids) return p.E == 1 && !p.shared;
+  return p.k > 0 && (long long)p.T * p.k <= kFewPairs;
+}
+
+// h [T k (+ T), stride] bfloat16 = act(s g) (s u) of the picked experts, pair by pair, then (shared) a row per token through matrix E; ids null: one
+// matrix, h [T, stride].  I: columns that exist; stride: I up to a multiple of 8; w_rows: twice I up to a multiple of 32.  wts: the pairs' s, or null.
+// clear [n_clear]: set to zero (the counters of the launch behind).
+SHARPI_EXPORT int sharpi_fp8_few_gated(const void* x, const void* x_scales, int kind, const void* w_codes, const void* w_scales, int w_rows, void* h,
+                                       int stride, const int* ids, const float* wts, int T, int k, int E, int shared, int I, int K, int act, float limit,
+                                       int R, int* clear, int n_clear, hipStream_t stream) {
+  if (T <= 0) return SHARPI_OK;
+  const F8Matrix W{(const uint8_t*)w_codes, (const uint8_t*)w_scales, w_rows, f8_blocks(K)};
+  const F8Picks pk{ids, wts, T, k, E, shared ? 1 : 0};
+  const GatedAct ga{act, limit};
+  if (I <= 0 || K <= 0 || w_rows != 2 * f8_padded_rows(I) || stride != (I + 7) / 8 * 8 || !act_known(ga) || !picks_ok(pk) ||
+      !matrix_ok(W, E + pk.shared) || !rows_ok(x, kind, T, K) || ((uintptr_t)h & 15)) return SHARPI_ERR_ARG;
+  const int mb = T <= 16 ? 1 : T <= 32 ? 2 : 4;
+  const int groups = ids ? (T * k < E ? T * k : E) + pk.shared : 1;
+  const dim3 grid((unsigned)ceil_div(I, 8 * R), (unsigned)groups), block(FW * kWave);
+#define FG(RV, MBV, XT) \
+  fp8_few_kernel<RV, MBV, XT, true><<<grid, block, 0, stream>>>(x, (const uint8_t*)x_scales, W, (bf16_t*)h, I, stride, T, K, ga, pk, clear, n_clear)
+#define FG_MB(RV, XT)        \
+  if (mb == 1) FG(RV, 1, XT); \
+  else if (mb == 2) FG(RV, 2, XT); \
+  else FG(RV, 4, XT)
+#define FG_X(RV)                                          \
+  if (kind == X_CODES) { FG_MB(RV, F8Codes); }            \
+  else if (mb == 1) FG(RV, 1, bf16_t);                    \
+  else return SHARPI_ERR_ARG
+  if (R == 2) { FG_X(2); }
+  else return SHARPI_ERR_ARG;
+#undef FG_X
+#undef FG_MB
+#undef FG
+  SHARPI_CHECK_LAUNCH();
+  return SHARPI_OK;
+}
+
+// out [T, N] bfloat16 = the sum over the picks of q(h row) W_e^T (times the pair's weight if wts is given), plus the always-on expert's.
+// h [T k (+ T), K]: bfloat16 (T <= 16, K a multiple of 8) or codes.  S shares of the blocks of k; part: S x tiles x 1 KB x R x row blocks; counters [tiles] zero.
+SHARPI_EXPORT int sharpi_fp8_few_sum(const void* h, const void* h_scales, int kind, const void* w_codes, const void* w_scales, int w_rows, void* out, const int* ids, const float* wts,
+                                     int T, int k, int E, int shared, int N, int K, int R, int S, void* part, int* counters, hipStream_t stream) {
+  if (T <= 0) return SHARPI_OK;
+  const F8Matrix W{(const uint8_t*)w_codes, (const uint8_t*)w_scales, w_rows, f8_blocks(K)};
+  const F8Picks pk{ids, wts, T, k, E, shared ? 1 : 0};
+  if (N <= 0 || K <= 0 || w_rows != f8_padded_rows(N) || !picks_ok(pk) || !matrix_ok(W, E + pk.shared) || !rows_ok(h, kind, T, K) || S < 1 ||
+      (S > 1 && (!part || !counters)) || (long long)(kFewPairs + 1) * W.U > 0x7fffffffLL) return SHARPI_ERR_ARG;
+  const int mb = T <= 16 ? 1 : T <= 32 ? 2 : 4;
+  const dim3 grid((unsigned)ceil_div(N, 16 * R), (unsigned)S), block(FW * kWave);
+#define FS(RV, MBV, XT) \
+  fp8_sum_kernel<RV, MBV, XT><<<grid, block, 0, stream>>>(h, (const uint8_t*)h_scales, W, (bf16_t*)out, N, K, pk, wts != nullptr, (f32x4*)part, counters)
+#define FS_MB(RV)            \
+  if (kind != X_CODES) FS(RV, 1, bf16_t); \
+  else if (mb == 1) FS(RV, 1, F8Codes); \
+  else if (mb == 2) FS(RV, 2, F8Codes); \
+  else FS(RV, 4, F8Codes)
+  if (R == 1) { FS_MB(1); }
+  else if (R == 2) { FS_MB(2); }
+  else return SHARPI_ERR_ARG;
+#undef FS_MB
+#undef FS
+  SHARPI_CHECK_LAUNCH();
+  return SHARPI_OK;
+}

@@ -1,0 +1,128 @@
+// Rows into 8-bit floating point (fp8.h holds the format), plain or behind a gated unit: x [M, K] -> codes [M, 128 U] and scale bytes
+// [M, 4 U4], or x [M, 2 K] (gate columns, then up columns) -> those of act(g) u rounded to x's type.
+//
+// Bound: a pass over memory (2 or 4 bytes in, 1 out).  16 neighbouring lanes hold a block of 128, eight values each: its largest
+// magnitude is found by register moves, nothing is read twice and nothing is kept.
+#include "fp8.h"
+
+// WIDE: rows of whole runs of eight from 16-byte addresses; else element by element.
+template <typename T, bool GATED, bool WIDE>
+__global__ __launch_bounds__(256) void fp8_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                                       long long n_blocks, int K, int U, int su, GatedAct act) {
+  const long long b = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (b >= n_blocks) return;                   // (16 lanes at once)
+  const int l = threadIdx.x & 15;
+  const long long row = b / U;
+  const int u = (int)(b - row * U), k = u * kF8Block + l * 8;
+  const T* src = x + row * (GATED ? 2 * (long long)K : K) + k;
+  float v[8];
+  if constexpr (WIDE) {
+    if (k < K) load8(src, v);
+    else
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_f32(src[i]) : 0.f;
+  }
+  if constexpr (GATED) {
+    float w[8];
+    if constexpr (WIDE) {
+      if (k < K) load8(src + K, w);
+      else
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = 0.f;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = k + i < K ? to_f32(src[K + i]) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(from_f32<T>(gated_f32(act, v[i], w[i], 1.f, false)));
+  }
+  uint32_t top = 0;
+  bool bad[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t m = __float_as_uint(v[i]) & 0x7fffffffu;
+    bad[i] = m >= 0x7f800000u;
+    if (!bad[i] && m > top) top = m;
+  }
+  float t = __uint_as_float(top);
+  t = fmaxf(t, row_rotated<8>(t));
+  t = fmaxf(t, row_rotated<4>(t));
+  t = fmaxf(t, row_rotated<2>(t));
+  t = fmaxf(t, row_rotated<1>(t));
+  const int s = f8_scale_of(__float_as_uint(t));
+  const float scale = f8_scale_value(s);
+  uint32_t c[2] = {f8_codes4(v[0], v[1], v[2], v[3], scale), f8_codes4(v[4], v[5], v[6], v[7], scale)};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (bad[i]) c[i / 4] = (c[i / 4] & ~(0xffu << (i % 4 * 8))) | kF8Nan << (i % 4 * 8);
+  *reinterpret_cast<uint2*>(codes + b * kF8Block + l * 8) = make_uint2(c[0], c[1]);
+  if (l == 0) scales[row * su + u] = (uint8_t)s;
+  else if (u == U - 1 && U - 1 + l < su) scales[row * su + U - 1 + l] = 127;      // (the bytes behind the last block: a scale of one)
+}
+
+// dtype of x (DT_*); act 0: x [M, K]; else the gated unit's code, x [M, 2K].
+SHARPI_EXPORT int sharpi_fp8_rows(const void* x, int dtype, void* codes, void* scales, int M, int K, int act, float limit, hipStream_t stream) {
+  if (M <= 0) return SHARPI_OK;
+  const GatedAct ga{act, limit};
+  if (K <= 0 || act < 0 || (act > 0 && !act_known(ga))) return SHARPI_ERR_ARG;
+  const int U = f8_blocks(K), su = f8_scale_stride(K);
+  const long long n = (long long)M * U;
+  if ((n + 15) / 16 > 0x7fffffffLL) return SHARPI_ERR_ARG;
+  const dim3 grid((unsigned)((n + 15) / 16)), block(256);
+  const bool wide = K % 8 == 0 && ((uintptr_t)x & 15) == 0;
+#define FR(T, G, W) fp8_rows_kernel<T, G, W><<<grid, block, 0, stream>>>((const T*)x, (uint8_t*)codes, (uint8_t*)scales, n, K, U, su, ga)
+#define FR_FORM(T)                                   \
+  if (act) { if (wide) FR(T, true, true); else FR(T, true, false); } \
+  else { if (wide) FR(T, false, true); else FR(T, false, false); }
+  if (dtype == DT_BF16) { FR_FORM(bf16_t) }
+  else if (dtype == DT_F32) { FR_FORM(float) }
+  else return SHARPI_ERR_ARG;
+#undef FR_FORM
+#undef FR
+  SHARPI_CHECK_LAUNCH();
+  return SHARPI_OK;
+}
+
+// out[t] = sum_j w[t, j] y[inv_pos[t, j]] (+ shared[t]) of bfloat16 rows, the sum in float; picks of n_experts and above have no row and add nothing.
+// Bound: a pass over the rows.
+template <bool WIDE>
+__global__ __launch_bounds__(256) void fp8_combine_kernel(const bf16_t* __restrict__ y, const int* __restrict__ inv_pos, const int* __restrict__ ids,
+                                                          const bf16_t* __restrict__ shared, const float* __restrict__ w, bf16_t* __restrict__ out,
+                                                          int columns, int k, int n_experts) {
+  constexpr int V = WIDE ? 8 : 1;
+  const size_t t = blockIdx.x;
+  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
+  if (c >= columns) return;
+  float acc[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = 0.f;
+  auto add = [&](const bf16_t* row, float weight) {
+    float v[V];
+    if constexpr (WIDE) load8(row + c, v);
+    else v[0] = to_f32(row[c]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = fmaf(weight, v[i], acc[i]);
+  };
+  for (int j = 0; j < k; ++j) {
+    const size_t p = t * k + j;
+    if (ids[p] < n_experts) add(y + (size_t)inv_pos[p] * columns, w ? w[p] : 1.f);
+  }
+  if (shared) add(shared + t * columns, 1.f);
+  if constexpr (WIDE) store8(out + t * columns + c, acc);
+  else out[t * columns + c] = f32_to_bf16(acc[0]);
+}
+
+SHARPI_EXPORT int sharpi_fp8_combine(const void* y, const int* inv_pos, const int* ids, const void* shared, const float* w, void* out, int n_tokens,
+                                     int columns, int k, int n_experts, hipStream_t stream) {
+  if (n_tokens <= 0) return SHARPI_OK;
+  if (columns <= 0 || k <= 0) return SHARPI_ERR_ARG;
+  const bool wide = columns % 8 == 0 && (((uintptr_t)y | (uintptr_t)out | (uintptr_t)shared) & 15) == 0;
+  const dim3 grid((unsigned)n_tokens, (unsigned)ceil_div(columns, wide ? 2048 : 256)), block(256);
+  if (wide) fp8_combine_kernel<true><<<grid, block, 0, stream>>>((const bf16_t*)y, inv_pos, ids, (const bf16_t*)shared, w, (bf16_t*)out, columns, k, n_experts);
+  else fp8_combine_kernel<false><<<grid, block, 0, stream>>>((const bf16_t*)y, inv_pos, ids, (const bf16_t*)shared, w, (bf16_t*)out, columns, k, n_experts);
+  SHARPI_CHECK_LAUNCH();
+  return SHARPI_OK;
+}

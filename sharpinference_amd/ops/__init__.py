@@ -2400,3 +2400,7 @@ def delta_chunks(proj: torch.Tensor, c_off: int, conv_w: torch.Tensor, ring: Opt
     out = torch.empty(proj.shape[0], nh * dv, dtype=torch.float32, device=proj.device)
     _run("sharpi_delta_chunks", *args, _ptr(chunks), _ptr(ents), n, _ptr(work), _ptr(out), _stream())
     return out
+
+
+from .fp8 import (FP8_BLOCK, FP8_FEW_ROWS, Fp8Rows, Fp8Weight, experts_fp8, feed_forward_fp8, fp8_weight, linear_fp8,  # noqa: E402
+                  quantize_rows, quantize_weight)

@@ -1,0 +1,338 @@
+"""Rows, products, feed-forwards and layers of routed experts in 8-bit floating point.
+
+A row is cut into blocks of 128 values; a block has one scale, a power of two 2^(s - 127) with the byte s from 1 to 247, the smallest with which
+the block's largest finite magnitude is at most 448; its values are stored as e4m3 (``torch.float8_e4m3fn``), rounded to nearest even.
+Infinities and NaN become NaN.  Weights are quantised by their rows (over k) when a program loads them, activations row by row in the call.  The matrix
+instruction applies both scales and adds in float; its results are offered as bfloat16 only, since of eight products on end it cuts those that
+are some 2^-13 of the largest.
+
+``x`` of a product is a bfloat16 or float32 tensor [M, K], or rows that ``quantize_rows`` made."""
+from __future__ import annotations
+
+import contextlib
+from typing import Optional, Union
+
+import torch
+
+from . import ACT_SILU, _code, _dev, _i32, _known_act_pair, _need, _ptr, _run, _stream, compute_units
+
+FP8_BLOCK = 128                # values that share a scale
+FP8_TILE = 32                  # weight rows of a stored tile
+FP8_FEW_ROWS = 64              # rows of the weight-streaming kernels (csrc/fp8_few.hip kFewRows)
+FP8_FEW_PAIRS = 1024           # (token, pick) pairs of the same (kFewPairs)
+FP8_MAX_EXPERTS = 1023         # experts of a layer, one more may be always on (kFewExperts, kMaxGroups)
+_X_CODES = 2                   # csrc/fp8_few.hip X_CODES
+
+
+def _blocks(k: int) -> int:
+    return -(-k // FP8_BLOCK)
+
+
+def _scale_stride(k: int) -> int:
+    return -(-_blocks(k) // 4) * 4
+
+
+def _padded(n: int) -> int:
+    return -(-n // FP8_TILE) * FP8_TILE
+
+
+def _powers(s: torch.Tensor) -> torch.Tensor:
+    """2^(s - 127) of scale bytes, exactly."""
+    return (s.int() << 23).view(torch.float32)
+
+
+def _device_of(t: torch.Tensor):
+    """The launches of a call go to its tensors' device."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _same_device(*ts) -> None:
+    first = ts[0].device
+    for t in ts:
+        _need(t is None or t.device == first, "operands must live on one device")
+
+
+class Fp8Rows:
+    """Rows [M, K] in 8 bits: ``codes`` float8_e4m3fn [M, K up to whole blocks of 128] (zeros behind K) and ``scales`` uint8 [M, blocks up to
+    a multiple of 4] (127 behind the last block).  ``values()`` gives what they stand for."""
+
+    __slots__ = ("codes", "scales", "shape")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, k: int):
+        _need(codes.dim() == 2 and codes.dtype == torch.float8_e4m3fn and codes.shape[1] == _blocks(k) * FP8_BLOCK,
+              "Fp8Rows: codes must be float8_e4m3fn [M, K up to whole blocks]")
+        _need(scales.dtype == torch.uint8 and tuple(scales.shape) == (codes.shape[0], _scale_stride(k)) and scales.device == codes.device,
+              "Fp8Rows: scales must be uint8 [M, blocks up to a multiple of 4] beside the codes")
+        self.codes, self.scales, self.shape = codes, scales, (codes.shape[0], int(k))
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def values(self) -> torch.Tensor:
+        M, k = self.shape
+        s = _powers(self.scales[:, :_blocks(k)])
+        return (self.codes.float().view(M, _blocks(k), FP8_BLOCK) * s[..., None]).reshape(M, -1)[:, :k]
+
+
+class Fp8Weight:
+    """A matrix [N, K] (or a stack [E, N, K]) in 8 bits, in the order the kernels read it: ``codes`` uint8 [(E,) tiles of 32 rows, blocks, 4096] and
+    ``scales`` uint8 [(E,) tiles, blocks / 4, 32, 4].  ``gated``: N = 2 I, gate rows then up rows, each half in tiles of its own."""
+
+    __slots__ = ("codes", "scales", "shape", "gated")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, gated: bool):
+        self.codes, self.scales, self.shape, self.gated = codes, scales, tuple(shape), bool(gated)
+
+    def dim(self) -> int:
+        return len(self.shape)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def stored_rows(self) -> int:
+        """Rows of one matrix as they are stored, filled up with zeros."""
+        return 2 * _padded(self.shape[-2] // 2) if self.gated else _padded(self.shape[-2])
+
+    def select(self, e: int) -> "Fp8Weight":
+        """Matrix e of a stack (a view)."""
+        return Fp8Weight(self.codes[e], self.scales[e], self.shape[1:], self.gated)
+
+    def values(self) -> torch.Tensor:
+        """float32 [(E,) N, K]: what the codes stand for (a copy, for tests and other kernels)."""
+        if self.dim() == 3:
+            return torch.stack([self.select(e).values() for e in range(self.shape[0])])
+        N, K = self.shape
+        R, U = self.stored_rows, _blocks(K)
+        c = self.codes.view(torch.float8_e4m3fn).view(R // 32, U, 2, 2, 2, 32, 16).float().permute(0, 5, 1, 2, 4, 3, 6).reshape(R, U, FP8_BLOCK)
+        s = self.scales.permute(0, 2, 1, 3).reshape(R, -1)[:, :U]
+        v = (c * _powers(s)[..., None]).reshape(R, -1)[:, :K]
+        return torch.cat([v[:N // 2], v[R // 2:R // 2 + N // 2]]) if self.gated else v[:N]
+
+
+def _pack(codes: torch.Tensor, scales: torch.Tensor, gated: bool, dst_codes: torch.Tensor, dst_scales: torch.Tensor) -> None:
+    """One matrix: codes uint8 [N, K], scales uint8 [N, blocks], into the stored order."""
+    (N, K), U = codes.shape, scales.shape[1]
+    R, U4 = dst_codes.shape[0] * FP8_TILE, dst_scales.shape[1]
+    rows, bytes_ = codes.new_zeros(R, U * FP8_BLOCK), scales.new_full((R, U4 * 4), 127)
+    for src, dst, n in ((0, 0, N // 2), (N // 2, R // 2, N // 2)) if gated else ((0, 0, N),):
+        rows[dst:dst + n, :K].copy_(codes[src:src + n])
+        bytes_[dst:dst + n, :U].copy_(scales[src:src + n])
+    # [tile, row, block, half, group, piece, 16] -> [tile, block, half, piece, group, row, 16]
+    dst_codes.view(R // 32, U, 2, 2, 2, 32, 16).copy_(rows.view(R // 32, 32, U, 2, 2, 2, 16).permute(0, 2, 3, 5, 4, 1, 6))
+    dst_scales.copy_(bytes_.view(R // 32, 32, U4, 4).permute(0, 2, 1, 3))
+
+
+def _new_weight(shape, gated: bool, device) -> Fp8Weight:
+    N, K = shape[-2:]
+    _need(len(shape) in (2, 3) and N > 0 and K > 0 and (len(shape) == 2 or 0 < shape[0] <= FP8_MAX_EXPERTS + 1),
+          f"8-bit weights must be [N, K] or [E, N, K] with at most {FP8_MAX_EXPERTS + 1} matrices")
+    _need(not gated or N % 2 == 0, "a gated matrix holds gate rows, then as many up rows")
+    R = 2 * _padded(N // 2) if gated else _padded(N)
+    _need(R * _blocks(K) <= 0x7fffffff, f"8-bit weights [{N}, {K}] are too large")
+    lead = tuple(shape[:-2])
+    return Fp8Weight(torch.empty(*lead, R // 32, _blocks(K), FP8_TILE * FP8_BLOCK, dtype=torch.uint8, device=device),
+                     torch.empty(*lead, R // 32, _scale_stride(K) // 4, FP8_TILE, 4, dtype=torch.uint8, device=device), shape, gated)
+
+
+def fp8_weight(codes: torch.Tensor, scales: torch.Tensor, gated: bool = False) -> Fp8Weight:
+    """A stored matrix in the kernels' order: codes float8_e4m3fn [(E,) N, K] and scales uint8 [(E,) N, K / 128 rounded up], the exponent bytes
+    (1 .. 254: 2^(s - 127)) of each row's blocks.  ``gated``: gate rows, then up rows of a feed-forward."""
+    _need(codes.dtype == torch.float8_e4m3fn and codes.dim() in (2, 3), "fp8_weight: codes must be float8_e4m3fn [N, K] or [E, N, K]")
+    _need(scales.dtype == torch.uint8 and tuple(scales.shape) == (*codes.shape[:-1], _blocks(codes.shape[-1])) and scales.device == codes.device,
+          "fp8_weight: scales must be uint8, one for each row's block of 128, beside the codes")
+    w = _new_weight(tuple(codes.shape), gated, codes.device)
+    if codes.dim() == 2:
+        _pack(codes.view(torch.uint8), scales, gated, w.codes, w.scales)
+    else:
+        for e in range(codes.shape[0]):
+            _pack(codes[e].view(torch.uint8), scales[e], gated, w.codes[e], w.scales[e])
+    return w
+
+
+def quantize_weight(w: torch.Tensor, gated: bool = False) -> Fp8Weight:
+    """A bfloat16 or float32 matrix [(E,) N, K] on the GPU in 8 bits (``quantize_rows`` of its rows), in the kernels' order."""
+    _need(w.is_cuda and w.dim() in (2, 3), "quantize_weight: a matrix [N, K] or a stack [E, N, K] on the GPU")
+    out = _new_weight(tuple(w.shape), gated, w.device)
+    for e in range(w.shape[0] if w.dim() == 3 else 1):
+        q = quantize_rows((w[e] if w.dim() == 3 else w).contiguous())
+        codes, scales = q.codes.view(torch.uint8)[:, :w.shape[-1]], q.scales[:, :_blocks(w.shape[-1])]
+        _pack(codes, scales, gated, out.codes[e] if w.dim() == 3 else out.codes, out.scales[e] if w.dim() == 3 else out.scales)
+    return out
+
+
+def _new_rows(M: int, k: int, device) -> Fp8Rows:
+    return Fp8Rows(torch.empty(M, _blocks(k) * FP8_BLOCK, dtype=torch.float8_e4m3fn, device=device),
+                   torch.empty(M, _scale_stride(k), dtype=torch.uint8, device=device), k)
+
+
+def quantize_rows(x: torch.Tensor, act=None) -> Fp8Rows:
+    """x [M, K] (bfloat16 or float32) in 8 bits; with ``act`` (ACT_SILU, ACT_GELU_TANH or (ACT_SWISH_CLAMP, limit)) x [M, 2I] holds gate
+    columns, then up columns, and the rows are act(g) * u, rounded to x's type first (what ``gated_act`` stores)."""
+    _dev(x)
+    _need(x.dim() == 2 and x.shape[1] > 0, "quantize_rows: x must be [M, K]")
+    dt = _code(x.dtype)
+    code, limit = (0, 0.0) if act is None else _known_act_pair(act)
+    _need(not code or x.shape[1] % 2 == 0, "quantize_rows: a gated input is [M, 2I]")
+    M, K = x.shape[0], x.shape[1] // (2 if code else 1)
+    out = _new_rows(M, K, x.device)
+    with _device_of(x):
+        _run("sharpi_fp8_rows", _ptr(x), dt, _ptr(out.codes), _ptr(out.scales), M, K, code, limit, _stream())
+    return out
+
+
+def _rows_of(x) -> Fp8Rows:
+    return x if isinstance(x, Fp8Rows) else quantize_rows(x)
+
+
+def _few_rows_of(x):
+    """(tensor, scales, kind) of the rows as the weight-streaming kernels take them: up to 16 rows of bfloat16 are quantised where they are read."""
+    if isinstance(x, Fp8Rows):
+        return x.codes, x.scales, _X_CODES
+    if x.dtype == torch.bfloat16 and x.shape[0] <= 16 and x.shape[1] % 8 == 0 and x.data_ptr() % 16 == 0:
+        return x, None, _code(x.dtype)
+    q = quantize_rows(x)
+    return q.codes, q.scales, _X_CODES
+
+
+def _rows_checked(x, k: int, who: str) -> None:
+    if isinstance(x, Fp8Rows):
+        _dev(x.codes, x.scales)
+    else:
+        _dev(x)
+        _code(x.dtype)
+    _need(len(x.shape) == 2 and x.shape[1] == k, f"{who}: x {tuple(x.shape)} does not fit weights over {k} columns")
+
+
+def linear_fp8(x: Union[torch.Tensor, Fp8Rows], w: Fp8Weight) -> torch.Tensor:
+    """x [M, K] W^T in 8 bits: bfloat16 [M, N]."""
+    _need(isinstance(w, Fp8Weight) and w.dim() == 2 and not w.gated, "linear_fp8: w must be an Fp8Weight [N, K], not gated")
+    N, K = w.shape
+    _rows_checked(x, K, "linear_fp8")
+    _same_device(w.codes, x if isinstance(x, torch.Tensor) else x.codes)
+    M = x.shape[0]
+    out = torch.empty(M, N, dtype=torch.bfloat16, device=w.device)
+    with _device_of(out):
+        if M <= FP8_FEW_ROWS:
+            rows, scales, kind = _few_rows_of(x)
+            _run("sharpi_fp8_few", _ptr(rows), _ptr(scales), kind, _ptr(w.codes), _ptr(w.scales), w.stored_rows, _ptr(out), M, N, K,
+                 _few_tiles(N), _stream())
+        else:
+            q = _rows_of(x)
+            _run("sharpi_fp8_tiles", _ptr(q.codes), _ptr(q.scales), M, _ptr(w.codes), _ptr(w.scales), w.stored_rows, _ptr(out), M, N, K,
+                 None, None, 1, 0, _height(M, 1), _stream())
+    return out
+
+
+def _few_tiles(N: int) -> int:
+    """Half tiles of 16 weight rows a block takes."""
+    return 2 if N >= 16384 else 1
+
+
+def _height(rows: int, groups: int) -> int:
+    """Rows of a tile."""
+    each = rows / groups
+    return 64 if each <= 64 else 128 if each <= 128 else 256
+
+
+def _layer_checked(x, w_gate_up: Fp8Weight, w_down: Fp8Weight, dims: int, who: str):
+    _need(isinstance(w_gate_up, Fp8Weight) and isinstance(w_down, Fp8Weight) and w_gate_up.dim() == w_down.dim() == dims
+          and w_gate_up.gated and not w_down.gated, f"{who}: w_gate_up must be a gated Fp8Weight and w_down a plain one, both {'[E, N, K]' if dims == 3 else '[N, K]'}")
+    inner, K = w_gate_up.shape[-2] // 2, w_gate_up.shape[-1]
+    _need(w_down.shape == (*w_gate_up.shape[:-2], w_down.shape[-2], inner), f"{who}: w_gate_up {w_gate_up.shape} and w_down {w_down.shape} do not fit")
+    _rows_checked(x, K, who)
+    _same_device(w_gate_up.codes, w_down.codes, x if isinstance(x, torch.Tensor) else x.codes)
+    return x.shape[0], K, inner, w_down.shape[-2]
+
+
+def _few_layer(x, ids, wts, w1: Fp8Weight, w2: Fp8Weight, code: int, limit: float, on_input: bool, shared: bool, E: int) -> torch.Tensor:
+    T, K, inner, N = x.shape[0], w1.shape[-1], w1.shape[-2] // 2, w2.shape[-2]
+    k = 1 if ids is None else ids.shape[1]
+    rows = T * k + (T if shared else 0)
+    stride = -(-inner // 8) * 8
+    R = 2
+    tiles = -(-N // (16 * R))
+    met = (min(E, T * k) + (1 if shared else 0)) if ids is not None else 1
+    S = max(1, min(2 * compute_units() // tiles, met * _blocks(inner) // 8))
+    row_blocks = 1 if T <= 16 else 2 if T <= 32 else 4
+    h = torch.empty(rows, stride, dtype=torch.bfloat16, device=w1.device)
+    out = torch.empty(T, N, dtype=torch.bfloat16, device=w1.device)
+    counters = torch.empty(tiles, dtype=torch.int32, device=w1.device)
+    part = torch.empty(S * tiles * R * row_blocks * 256 if S > 1 else 1, dtype=torch.float32, device=w1.device)
+    a, scales, kind = _few_rows_of(x)
+    w_in, w_out = (wts, None) if on_input else (None, wts)
+    _run("sharpi_fp8_few_gated", _ptr(a), _ptr(scales), kind, _ptr(w1.codes), _ptr(w1.scales), w1.stored_rows, _ptr(h), stride, _ptr(ids), _ptr(w_in),
+         T, k, E, 1 if shared else 0, inner, K, code, limit, 2, _ptr(counters), tiles, _stream())
+    if T <= 16:
+        a, scales, kind = h, None, _code(h.dtype)
+    else:
+        q = quantize_rows(h)
+        a, scales, kind = q.codes, q.scales, _X_CODES
+    _run("sharpi_fp8_few_sum", _ptr(a), _ptr(scales), kind, _ptr(w2.codes), _ptr(w2.scales), w2.stored_rows, _ptr(out), _ptr(ids), _ptr(w_out), T, k, E,
+         1 if shared else 0, N, stride, R, S, _ptr(part), _ptr(counters), _stream())
+    return out
+
+
+def feed_forward_fp8(x: Union[torch.Tensor, Fp8Rows], w_gate_up: Fp8Weight, w_down: Fp8Weight, act=ACT_SILU) -> torch.Tensor:
+    """A gated feed-forward in 8 bits: h = act(g) * u with (g | u) = x W_gate_up^T, rounded to bfloat16 and quantised again, then h W_down^T: bfloat16
+    [M, N].  A few rows: two launches (up to 16 rows of bfloat16; four up to 64); more: the quantised h is the first product's epilogue."""
+    M, K, inner, N = _layer_checked(x, w_gate_up, w_down, 2, "feed_forward_fp8")
+    code, limit = _known_act_pair(act)
+    with _device_of(w_down.codes):
+        if M == 0:
+            return torch.empty(0, N, dtype=torch.bfloat16, device=w_down.device)
+        if M <= FP8_FEW_ROWS:
+            return _few_layer(x, None, None, w_gate_up, w_down, code, limit, False, False, 1)
+        q, h = _rows_of(x), _new_rows(M, inner, w_down.device)
+        _run("sharpi_fp8_tiles_gated", _ptr(q.codes), _ptr(q.scales), M, _ptr(w_gate_up.codes), _ptr(w_gate_up.scales), w_gate_up.stored_rows, _ptr(h.codes),
+             _ptr(h.scales), M, inner, K, None, None, 1, 0, None, code, limit, _height(M, 1), _stream())
+        return linear_fp8(h, w_down)
+
+
+def experts_fp8(x: Union[torch.Tensor, Fp8Rows], ids: torch.Tensor, wts: torch.Tensor, w_gate_up: Fp8Weight, w_down: Fp8Weight, act=ACT_SILU,
+                score_on_input: bool = False, shared: bool = False) -> torch.Tensor:
+    """A layer of routed experts in 8 bits, whole: out[t] = sum_j wts[t, j] F_e(x[t]) over the token's picks e = ids[t, j], with F_e the gated
+    feed-forward of matrix e (see ``feed_forward_fp8``); with ``score_on_input`` the pick's score multiplies g and u instead.  ``shared``: the stacks hold
+    one more matrix behind the experts, whose feed-forward of every token is added.  ids int32 [T, k] and wts float32 [T, k] as the router
+    gives them (``router_topk``); a pick of the experts' number or above adds nothing, negative ones are not allowed.  bfloat16 [T, N].
+
+    Up to 64 tokens the picks are taken as they are: two launches for up to 16 rows of bfloat16 (four beyond), the second of which adds the experts' outputs in float.  More
+    tokens are sorted by expert; a pick's output is then rounded to bfloat16 before the sum."""
+    T, K, inner, N = _layer_checked(x, w_gate_up, w_down, 3, "experts_fp8")
+    _dev(ids, wts)
+    _i32(ids, "ids")
+    _need(ids.dim() == 2 and ids.shape[0] == T and ids.shape[1] > 0 and wts.shape == ids.shape and wts.dtype == torch.float32,
+          "experts_fp8: ids must be int32 and wts float32 [T, k]")
+    _same_device(w_down.codes, ids, wts)
+    E, k = w_gate_up.shape[0] - (1 if shared else 0), ids.shape[1]
+    _need(0 < E <= FP8_MAX_EXPERTS and k <= FP8_FEW_PAIRS, f"experts_fp8: up to {FP8_MAX_EXPERTS} experts and {FP8_FEW_PAIRS} picks")
+    code, limit = _known_act_pair(act)
+    with _device_of(w_down.codes):
+        if T == 0:
+            return torch.empty(0, N, dtype=torch.bfloat16, device=w_down.device)
+        if T <= FP8_FEW_ROWS and T * k <= FP8_FEW_PAIRS:
+            return _few_layer(x, ids, wts, w_gate_up, w_down, code, limit, score_on_input, shared, E)
+        return _many_layer(_rows_of(x), ids, wts, w_gate_up, w_down, code, limit, score_on_input, shared, E, inner, N)
+
+
+def _many_layer(q: Fp8Rows, ids, wts, w1: Fp8Weight, w2: Fp8Weight, code: int, limit: float, on_input: bool, shared: bool, E: int, inner: int, N: int) -> torch.Tensor:
+    T, k = ids.shape
+    n, along, dev = T * k, T if shared else 0, w1.device
+    # the picks sorted by expert (no plan: that is the bfloat16 product's); the always-on matrix takes the tokens behind them, in their order
+    ints = torch.empty(E + 1 + 2 * n, dtype=torch.int32, device=dev)
+    offsets, tokens, inv_pos = ints[:E + 1], ints[E + 1:E + 1 + n], ints[E + 1 + n:]
+    scores = torch.empty(n, dtype=torch.float32, device=dev)
+    _run("sharpi_moe_permute", _ptr(ids), _ptr(wts), _ptr(offsets), _ptr(tokens), _ptr(scores), _ptr(inv_pos), None, 0, T, k, E, 0, 1, _stream())
+    height = _height(n, E)
+    h = _new_rows(n + along, inner, dev)
+    _run("sharpi_fp8_tiles_gated", _ptr(q.codes), _ptr(q.scales), T, _ptr(w1.codes), _ptr(w1.scales), w1.stored_rows, _ptr(h.codes), _ptr(h.scales),
+         n, inner, w1.shape[-1], _ptr(tokens), _ptr(offsets), E, along, _ptr(scores) if on_input else None, code, limit, height, _stream())
+    y = torch.empty(n + along, N, dtype=torch.bfloat16, device=dev)
+    _run("sharpi_fp8_tiles", _ptr(h.codes), _ptr(h.scales), n + along, _ptr(w2.codes), _ptr(w2.scales), w2.stored_rows, _ptr(y), n, N, inner,
+         None, _ptr(offsets), E, along, height, _stream())
+    out = torch.empty(T, N, dtype=torch.bfloat16, device=dev)
+    _run("sharpi_fp8_combine", _ptr(y), _ptr(inv_pos), _ptr(ids), _ptr(y[n:]) if shared else None, None if on_input else _ptr(wts), _ptr(out),
+         T, N, k, E, _stream())
+    return out
