@@ -35,6 +35,12 @@ __device__ __forceinline__ void load_to_lds(u32x4 rsrc, uint32_t offset, uint32_
   else
     asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"{m0}"(lds), "v"(offset), "s"(rsrc), "s"(step) : "memory");
 }
+// Lane l's 4 bytes, to LDS byte lds + 4 l.
+__device__ __forceinline__ void load_words_to_lds(u32x4 rsrc, uint32_t offset, uint32_t step, uint32_t lds) {
+  lds = __builtin_amdgcn_readfirstlane(lds);
+  step = __builtin_amdgcn_readfirstlane(step);
+  asm volatile("s_nop 4\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"{m0}"(lds), "v"(offset), "s"(rsrc), "s"(step) : "memory");
+}
 // Two such loads by one descriptor and step, to two places: the wait states ahead of both once, and between them m0 written and the one
 // state behind that.  m0 is written before the second load reads step, descriptor and offset: early (&), or a step that equals lds0 is read
 // out of it.  us of products, a load at a time and in pairs: 64 experts of 2,816 x 2,048, six picks, 1,664 tokens 197 -> 192; 28 of 2,048 x
