@@ -60,6 +60,22 @@ __device__ __forceinline__ uint32_t f8_codes4(uint32_t lo, uint32_t hi, float sc
   v = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(v, __builtin_bit_cast(bf16x2v_t, hi), scale, true);
   return __builtin_bit_cast(uint32_t, v);
 }
+// act(g) u of a gated feed-forward whose result is rounded to bfloat16 and quantised: each of the activations is g times a logistic function
+// (tanh-GELU's 0.5 (1 + tanh z) is that of 2 z), by the hardware's power of two and reciprocal: 2^-22 of the result, and 2^-23 |z| of it
+// from the exponent, where the general exponential and division take some 30 instructions an element.
+template <int ACT> __device__ __forceinline__ float f8_unit(float limit, float g, float u) {
+  if constexpr (ACT == ACT_SWISH_CLAMP) {
+    g = fminf(g, limit);
+    u = fminf(fmaxf(u, -limit), limit) + 1.0f;
+  }
+  const float z = ACT == ACT_SWISH_CLAMP ? kSwishSlope * g : ACT == ACT_GELU_TANH ? 1.5957691216057308f * (g + 0.044715f * g * g * g) : g;
+  return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z)) * u;
+}
+__device__ __forceinline__ float f8_unit(GatedAct act, float g, float u) {
+  if (act.code == ACT_SWISH_CLAMP) return f8_unit<ACT_SWISH_CLAMP>(act.limit, g, u);
+  if (act.code == ACT_GELU_TANH) return f8_unit<ACT_GELU_TANH>(act.limit, g, u);
+  return f8_unit<ACT_SILU>(act.limit, g, u);
+}
 struct MaxBits {    // the larger of two magnitudes by their bits (NaN is the largest, not lost)
   __device__ __forceinline__ float operator()(float a, float b) const {
     const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);

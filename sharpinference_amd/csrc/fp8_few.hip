@@ -269,7 +269,7 @@ __global__ __launch_bounds__(FW* kWave, 4) void fp8_few_kernel(const void* __res
             const float sc = scaled ? pk.w[orow] : 1.0f;
             f32x4 o;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = gated_f32(act, gv[i], uv[i], sc, scaled);
+            for (int i = 0; i < 4; ++i) o[i] = f8_unit(act, gv[i] * sc, uv[i] * sc);
             store_columns(out + (size_t)orow * stride, n, stride, o);
           }
         }

@@ -28,6 +28,7 @@ struct F8Tiles {
   int rows, groups;          // rows of the sorted list at most
   uint32_t x_bytes;          // of x's codes (with a_rows)
   int along;                 // rows behind these that one more matrix takes, in the order of x (0: none)
+  int height;                // rows of a tile at most, a multiple of 64
   int tiles, nb;             // row tiles in all at most; column blocks
 };
 
@@ -40,66 +41,38 @@ struct F8Out {
   int n_out;
 };
 
-// Where 16-byte piece `piece` of row `row` of a stage is kept: the pieces of a wave's read fall into different 16-byte groups of the banks.
-__device__ __forceinline__ int row_piece(int row, int piece) { return piece ^ ((row >> 1) & 7); }
+// Where 16-byte piece `piece` of row `row` of a step is kept: the pieces that sixteen neighbouring lanes read fall into the sixteen 16-byte groups
+// of the banks.
+__device__ __forceinline__ int row_piece(int row, int piece) { return piece ^ ((row >> 2) & 3); }
 
-// MT: groups of 32 rows a wave; a tile has 64 MT rows.
+// LDS holds a ring of slots, a slot one step (64 of k: 16 KB of weights, 4 KB of rows for each MT) of tall tiles, or two steps of tiles of up to 128 rows,
+// whose steps are short beside a barrier.
+constexpr int slot_steps(int mt) { return mt <= 2 ? 2 : 1; }
+constexpr int slots(int mt) { return mt <= 2 ? 3 : 4; }
+constexpr int kWStep = 16384;
+constexpr int step_bytes(int mt) { return kWStep + 4096 * mt; }
+constexpr int scales_at(int mt) { return slots(mt) * slot_steps(mt) * step_bytes(mt); }
+constexpr int kTileLds = scales_at(2) + 3 * 2048;
+static_assert(scales_at(4) <= scales_at(2) && scales_at(3) <= scales_at(2) && scales_at(1) <= scales_at(2), "the largest ring");
+constexpr int kHighest = 4;            // a tile has up to 64 x this many rows
+
+// One tile: rows row0 .. row_end (up to 64 MT of them) of matrix e against column block nblock.  MT: groups of 32 rows a wave.
 template <int MT, bool GATED>
-__global__ __launch_bounds__(TW* kWave, 2) void fp8_tiles_kernel(F8Tiles p, F8Out o, GatedAct act) {
-  constexpr int TM = 64 * MT;
-  // The rings: of tall tiles two stages of rows (128 of k) and four steps of weights (64 of k), filled a step at a time, weights three steps ahead; of
-  // tiles of up to 128 rows, whose steps are short beside a latency, three stages of both, filled a stage at a time.
-  constexpr bool STAGED = MT <= 2;
-  constexpr int RS = STAGED ? 3 : 2;
-  constexpr int kWStep = 16384, kXStage = TM * kF8Block, kXAt = 2 * RS * kWStep, kSAt = kXAt + RS * kXStage;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[kSAt + 3 * 2048];
-  __shared__ int s_offset[kMaxGroups + 1];
-  __shared__ int s_group, s_row0, s_end;
-  __shared__ float s_top[TWC][GATED ? TM : 1];
+__device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedAct act, int e, int row0, int row_end, int nblock, unsigned char* smem,
+                                        float (*s_top)[64 * kHighest]) {
+  constexpr int NS = slot_steps(MT), RING = slots(MT) * NS, AHEAD = RING - NS;      // (steps)
+  constexpr int kStep = step_bytes(MT), kSAt = scales_at(MT);
   const int lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 31, g = lane >> 5;
   const int wr = wid / TWC, wc = wid % TWC;
-  const int tile = blockIdx.x % p.tiles, nblock = blockIdx.x / p.tiles;
-  int e = 0, row0 = tile * TM, row_end = min(p.rows, row0 + TM);
-  if (p.offsets) {
-    for (int i = threadIdx.x; i <= p.groups; i += TW * kWave) s_offset[i] = p.offsets[i];
-    if (threadIdx.x == 0) s_group = -1;
-    __syncthreads();
-    if (wid == 0) {
-      int before = 0;
-      for (int c = 0; c < p.groups + (p.along > 0); c += kWave) {
-        const int i = c + lane;
-        const int from = i < p.groups ? s_offset[i] : p.rows, to = i < p.groups ? s_offset[i + 1] : i == p.groups ? p.rows + p.along : p.rows;
-        const int mine = (to - from + TM - 1) / TM;
-        int upto = mine;
-#pragma unroll
-        for (int k = 1; k < kWave; k <<= 1) {
-          const int up = __shfl_up(upto, k, kWave);
-          if (lane >= k) upto += up;
-        }
-        const int first = before + upto - mine;
-        if (mine > 0 && tile >= first && tile < first + mine) {
-          s_group = i;
-          s_row0 = from + (tile - first) * TM;
-          s_end = min(to, s_row0 + TM);
-        }
-        before += __shfl(upto, kWave - 1, kWave);
-      }
-    }
-    __syncthreads();
-    if (s_group < 0) return;
-    e = __builtin_amdgcn_readfirstlane(s_group);
-    row0 = __builtin_amdgcn_readfirstlane(s_row0);
-    row_end = __builtin_amdgcn_readfirstlane(s_end);
-  }
   const bool sorted = row0 < p.rows;             // of the sorted list, not of the rows behind it
   const int U4 = (p.U + 3) >> 2;
   const int half = p.w_rows / 64;                // gated: tiles of the gate rows
   const bool exists = !GATED || nblock * (kTileCols / 64) + wc < half;
-  // Loads into LDS.  Weights: wave wid brings tile wid of the block's eight (gated: a wave column's gate tile, then its up tile), a step of 64 of k
-  // is 2 KB of it on end.  Rows: a load brings 8 rows of 128 bytes (a stage: two steps), lane l row l / 8 at place l % 8, their 16-byte pieces
-  // exchanged by row bits (row_piece).  Rows behind the last read it again; what they give is never stored.  Scales: a chunk of four blocks of k
-  // is a word a row; waves 0 to 3 bring those of 64 rows each, waves 4 to 7 those of two weight tiles each.
+  // Loads go straight into LDS.  Weights: wave wid brings tile wid of the block's eight (gated: a wave column's gate tile, then its up tile), a step is
+  // 2 KB of it on end.  Rows: a load brings 16 rows of 64 bytes, their 16-byte pieces exchanged by row bits (row_piece).  Rows behind the last read it
+  // again; what they give is never stored.  Scales: a chunk of four blocks of k is a word a row; waves 0 to 3 bring those of 64 rows each,
+  // waves 4 to 7 those of two weight tiles each.
   auto block_tile = [&](int lt) {
     if constexpr (GATED) return min(nblock * (kTileCols / 64) + lt / 2, half - 1) + lt % 2 * half;
     else return min(nblock * (kTileCols / 32) + lt, p.w_rows / 32 - 1);
@@ -115,20 +88,19 @@ __global__ __launch_bounds__(TW* kWave, 2) void fp8_tiles_kernel(F8Tiles p, F8Ou
     const int row = min(row0 + lrow, row_end - 1);
     return !p.a_rows ? row - row0 : sorted ? p.a_rows[row] : row - p.rows;
   };
-  constexpr int XL = MT;                                  // loads of rows a wave and stage
+  constexpr int XL = (MT + 1) / 2;                        // loads of rows a wave and step (of 4 MT; some twice, to the same place)
   const int steps = 2 * p.U;
   const uint32_t w_off[2] = {(uint32_t)lane * 16, (uint32_t)lane * 16 + 1024};
-  auto load_w = [&](int s, int place) {
-    const uint32_t at[2] = {lds0 + place * kWStep + wid * 2048, lds0 + place * kWStep + wid * 2048 + 1024};
-    load_two_to_lds<false>(wb, w_off[0], w_off[1], min(s, steps - 1) * 2048, at[0], at[1]);
+  auto load_w = [&](int s, uint32_t at) {                 // (past the end: the last step once more, for nobody)
+    load_two_to_lds<false>(wb, w_off[0], w_off[1], min(s, steps - 1) * 2048, lds0 + at + wid * 2048, lds0 + at + wid * 2048 + 1024);
   };
-#pragma unroll
-  for (int s = 0; s < (STAGED ? 2 * RS - 2 : 3); ++s) load_w(s, s);      // (on their way while the rows' places are looked up)
   uint32_t x_off[XL], xs_off;
+  int x_to[XL];
 #pragma unroll
   for (int i = 0; i < XL; ++i) {
-    const int lrow = (wid * XL + i) * 8 + (lane >> 3);
-    x_off[i] = (uint32_t)x_row(lrow) * x_stride + row_piece(lrow, lane & 7) * 16;
+    const int li = (wid * XL + i) % (4 * MT), lrow = li * 16 + (lane >> 2);
+    x_to[i] = kWStep + li * 1024;
+    x_off[i] = (uint32_t)x_row(lrow) * x_stride + row_piece(lrow, lane & 3) * 16;
   }
   // scales: the wave's own buffer
   u32x4 sb;
@@ -154,15 +126,18 @@ __global__ __launch_bounds__(TW* kWave, 2) void fp8_tiles_kernel(F8Tiles p, F8Ou
   asm volatile("" : "+v"(xs_off));
   // the scales of the chunk behind chunk c, once a chunk; the other blocks' loads go where nobody reads
   auto load_s = [&](int c, bool first) { load_words_to_lds(sb, xs_off, min(c + 1, U4 - 1) * s_step, s_lds + (first ? ((c + 1) & 1) * 2048 : 4096)); };
-  auto load_x = [&](int c, int place) {
-    uint32_t at[XL];
+  auto load_x = [&](int s, uint32_t at) {
+    uint32_t to[XL];
 #pragma unroll
-    for (int i = 0; i < XL; ++i) at[i] = lds0 + kXAt + place * kXStage + (wid * XL + i) * 1024;
-    bring_all_to_lds<true, XL>(xb, x_off, min(c, p.U - 1) * kF8Block, at);
+    for (int i = 0; i < XL; ++i) to[i] = lds0 + at + x_to[i];
+    bring_all_to_lds<true, XL>(xb, x_off, min(s, steps - 1) * 64, to);
   };
   load_s(-1, true);
 #pragma unroll
-  for (int c = 0; c < RS - 1; ++c) load_x(c, c);
+  for (int s = 0; s < AHEAD; ++s) {
+    load_w(s, s * kStep);
+    load_x(s, s * kStep);
+  }
 
   f32x16 acc[2][MT];
 #pragma unroll
@@ -171,184 +146,251 @@ __global__ __launch_bounds__(TW* kWave, 2) void fp8_tiles_kernel(F8Tiles p, F8Ou
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[t][m][i] = 0.f;
-  // operand addresses: piece q of a lane's 32 bytes of half hh
-  int w_lds[2], x_lds[2][2];
+  // operand addresses: W of the step, and piece q of a lane's 32 bytes of its rows
+  int w_lds = wc * 4096 + lane * 16, x_lds[2];
 #pragma unroll
-  for (int hh = 0; hh < 2; ++hh) {
-    w_lds[hh] = wc * 4096 + lane * 16 + hh * kWStep;
-#pragma unroll
-    for (int q = 0; q < 2; ++q) x_lds[hh][q] = kXAt + (wr * MT * 32 + r) * 128 + row_piece(r, hh * 4 + g * 2 + q) * 16;
-  }
+  for (int q = 0; q < 2; ++q) x_lds[q] = kWStep + (wr * MT * 32 + r) * 64 + row_piece(r, g * 2 + q) * 16;
   const int ws_lds = kSAt + 1024 + wc * 256 + r * 4, xs_lds = kSAt + (wr * MT * 32 + r) * 4;
   constexpr int H0 = (MT + 1) / 2, H1 = MT / 2;
-  i32x8 wf[2][2], x0[H0], x1[H1 > 0 ? H1 : 1];
+  i32x8 wf[2], x0[H0], x1[H1 > 0 ? H1 : 1];
   int bw[2], bx[MT];                               // the block's scales
-  int place = 0;
-  // Every step sends the same loads, past the end too (the last step once more, into places that nobody reads any more): the waits count
-  // them, and there is no branch in the loop.  (With branches around them the products of two steps ended up behind the loads: 256 registers, spilled.)
-  auto arrive = [&](auto half_tag) {               // the next step is in LDS, and everyone has read the one before
-    constexpr int hh = decltype(half_tag)::value;
-    if constexpr (STAGED) {
-      if (hh == 1) return;
-      lds_loads_wait<XL + 5>();                    // a stage behind this one's loads
-    } else {
-      lds_loads_wait<hh == 0 ? 4 : 5 + XL>();      // two steps of weights and, in a stage's second step, the next stage's rows and scales
-    }
-    __syncthreads();
-  };
-  auto send = [&](int s, auto half_tag) {          // the loads that take the place of step s - 1, or of the stage before
-    constexpr int hh = decltype(half_tag)::value;
-    const int u = s >> 1;
-    if constexpr (hh == 0) load_s(u >> 2, (u & 3) == 0);
-    if constexpr (STAGED) {
-      if constexpr (hh == 0) {
-        const int c = u + RS - 1, to = place == 0 ? RS - 1 : place - 1;
-        load_x(c, to);
-        load_w(2 * c, 2 * to);
-        load_w(2 * c + 1, 2 * to + 1);
-      }
-    } else {
-      if constexpr (hh == 0) load_x(u + 1, place ^ 1);
-      load_w(s + 3, (s + 3) & 3);
-    }
-  };
   auto operand = [&](int a, int b) {
     const i32x4 lo = *reinterpret_cast<const i32x4*>(smem + a), hi = *reinterpret_cast<const i32x4*>(smem + b);
     return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
-  auto read_first = [&](auto half_tag) {
-    constexpr int hh = decltype(half_tag)::value;
+  auto read_w = [&](i32x8 (&to)[2]) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) wf[hh][t] = operand(w_lds[hh] + t * 2048, w_lds[hh] + t * 2048 + 1024);
-#pragma unroll
-    for (int m = 0; m < H0; ++m) x0[m] = operand(x_lds[hh][0] + m * 4096, x_lds[hh][1] + m * 4096);
+    for (int t = 0; t < 2; ++t) to[t] = operand(w_lds + t * 2048, w_lds + t * 2048 + 1024);
   };
-  auto in_turn = [&](auto reads_tag, auto products_tag) {
-    constexpr int R = decltype(reads_tag)::value, P = decltype(products_tag)::value, kEach = R > 0 && P > 0 ? (R + P - 1) / P : 1;
+  auto read_rows = [&](i32x8* to, int m0, int n) {
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
-      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-    }
+    for (int m = 0; m < n; ++m) to[m] = operand(x_lds[0] + (m0 + m) * 2048, x_lds[1] + (m0 + m) * 2048);
   };
-  auto step = [&](int s, auto half_tag, auto last_tag) {
+  auto read_scales = [&](int u, int (&w)[2], int (&x)[MT]) {
+    const int at = (u & 3) + (u >> 2 & 1) * 2048;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) w[t] = smem[ws_lds + t * 128 + at];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) x[m] = smem[xs_lds + m * 128 + at];
+  };
+  int at = 0;                                      // this step's bytes in the ring
+  auto ahead = [&](int n) {                        // those of n steps on
+    const int a = at + n * kStep;
+    return (uint32_t)(a >= RING * kStep ? a - RING * kStep : a);
+  };
+  // A step.  Its weights and first row groups are in registers; it reads the others while the first are multiplied, and the next step's
+  // first part, behind the barrier, while the others are.  The loads AHEAD steps on go out one by one among the products (a wave that
+  // sends all of a stage's on end stands still until the memory pipe has taken them).  Every step sends the same loads, so that the waits
+  // count them and the loop has no branch (with branches around them the products of two steps ended up behind the loads: 256 registers, spilled).
+  auto step = [&](int s, auto half_tag) {
     constexpr int hh = decltype(half_tag)::value;
-    constexpr bool last = decltype(last_tag)::value;
-    if constexpr (hh == 0) {
-      const int at = (s >> 1 & 3) + (s >> 3 & 1) * 2048;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) bw[t] = smem[ws_lds + t * 128 + at];
-#pragma unroll
-      for (int m = 0; m < MT; ++m) bx[m] = smem[xs_lds + m * 128 + at];
-    }
-#pragma unroll
-    for (int m = 0; m < H1; ++m) x1[m] = operand(x_lds[hh][0] + (H0 + m) * 4096, x_lds[hh][1] + (H0 + m) * 4096);
     auto row_products = [&](const i32x8& rows, int m) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) acc[t][m] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[hh][t], rows, acc[t][m], 0, 0, 0, bw[t], 0, bx[m]);
+      for (int t = 0; t < 2; ++t) acc[t][m] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[t], rows, acc[t][m], 0, 0, 0, bw[t], 0, bx[m]);
     };
+    if constexpr (H1 > 0) read_rows(x1, H0, H1);
+    row_products(x0[0], 0);
+    __builtin_amdgcn_sched_barrier(0);
+    load_x(s + AHEAD, ahead(AHEAD));
+    if constexpr (hh == 0) load_s(s >> 3, (s & 6) == 0);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int m = 0; m < H0; ++m) row_products(x0[m], m);
-    in_turn(std::integral_constant<int, 2 * H1>{}, std::integral_constant<int, 2 * H0>{});
+    for (int m = 1; m < H0; ++m) row_products(x0[m], m);
+    __builtin_amdgcn_sched_barrier(0);             // products of the first row groups stay ahead of the barrier, those of the others behind it
+    if constexpr (NS == 1 || hh == 1) {
+      // the next slot is here, and everyone has read the one before: counted are the slots behind it (a scales' load among them makes the wait one longer)
+      lds_loads_wait<NS == 1 ? 2 * (2 + XL) : 2 * (2 + XL)>();
+      __syncthreads();
+    }
+    const int turn = at == (RING - 1) * kStep ? (1 - RING) * kStep : kStep;
+    at += turn;
+    w_lds += turn;
+    x_lds[0] += turn;
+    x_lds[1] += turn;
+    __builtin_amdgcn_sched_barrier(0);
+    i32x8 wn[2];
+    int nw[2], nx[MT];
+    if constexpr (hh == 1) read_scales((s + 1) >> 1, nw, nx);
+    read_w(wn);
+    read_rows(x0, 0, H0);
+    if constexpr (H1 > 0) row_products(x1[0], H0);
+    __builtin_amdgcn_sched_barrier(0);
+    load_w(s + 1 + AHEAD, ahead(AHEAD));
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int m = 1; m < H1; ++m) row_products(x1[m], H0 + m);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) wf[t] = wn[t];
     if constexpr (hh == 1) {
-      const int turn = place == RS - 1 ? 1 - RS : 1;
-      place += turn;
-      w_lds[0] += turn * 2 * kWStep;
-      w_lds[1] += turn * 2 * kWStep;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x_lds[i / 2][i % 2] += turn * kXStage;
-    }
-    if constexpr (!last) {
-      __builtin_amdgcn_sched_barrier(0);           // products of the first half stay ahead of the barrier, those of the other behind it
-      arrive(std::integral_constant<int, hh ^ 1>{});
-      __builtin_amdgcn_sched_barrier(0);
-      read_first(std::integral_constant<int, hh ^ 1>{});
-    }
-    constexpr int kBefore = H1 / 2;
+      for (int t = 0; t < 2; ++t) bw[t] = nw[t];
 #pragma unroll
-    for (int m = 0; m < kBefore; ++m) row_products(x1[m], H0 + m);
-    if constexpr (!last) {
-      in_turn(std::integral_constant<int, 4 + 2 * H0>{}, std::integral_constant<int, kBefore * 2>{});
-      __builtin_amdgcn_sched_barrier(0);
-      send(s + 1, std::integral_constant<int, hh ^ 1>{});
-      __builtin_amdgcn_sched_barrier(0);
+      for (int m = 0; m < MT; ++m) bx[m] = nx[m];
     }
-#pragma unroll
-    for (int m = kBefore; m < H1; ++m) row_products(x1[m], H0 + m);
   };
-  using Half0 = std::integral_constant<int, 0>;
-  using Half1 = std::integral_constant<int, 1>;
   lds_loads_wait<0>();
   __syncthreads();
-  send(0, Half0{});
-  read_first(Half0{});
-  for (int u = 0; u + 1 < p.U; ++u) {
-    step(2 * u, Half0{}, std::false_type{});
-    step(2 * u + 1, Half1{}, std::false_type{});
+  read_scales(0, bw, bx);
+  read_w(wf);
+  read_rows(x0, 0, H0);
+  load_w(AHEAD, AHEAD * kStep);
+  for (int s = 0; s < steps; s += 2) {
+    step(s, std::integral_constant<int, 0>{});
+    step(s + 1, std::integral_constant<int, 1>{});
   }
-  step(steps - 2, Half0{}, std::false_type{});
-  step(steps - 1, Half1{}, std::true_type{});
   lds_loads_wait<0>();
   // a lane holds, of row row0 + (wr MT + m) 32 + r, columns 8 q + 4 g + 0..3 (q 0..3) of tile t
   if constexpr (!GATED) {
+    const int n_base = nblock * kTileCols + wc * 64;
+    if (n_base >= o.n_out) return;
+    // The results go through the wave's own part of LDS (everyone has read the last step), a row group at a time, to leave as whole lines of 128 bytes;
+    // a lane first exchanges halves with lane ^ 32, so that it has eight columns of its row.  Rows that do not begin at 16-byte addresses are
+    // stored by elements.  (Stored from the registers, pieces of 16 bytes a row, 8,192 x 2,048 x 2,560 in one round of tiles took 49 us, so 39.)
+    const bool wide = (o.n_out & 7) == 0 && ((uintptr_t)o.out & 15) == 0;
+    __syncthreads();
+    unsigned char* mine = smem + wid * 4096;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const int row = row0 + (wr * MT + m) * 32 + r;
-      if (row >= row_end) continue;
+      const int first = row0 + (wr * MT + m) * 32;
+      if (first >= row_end) break;                  // (the wave's)
+      if (wide) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int n = nblock * kTileCols + wc * 64 + t * 32 + q * 8 + g * 4;
-          bf16_t* dst = o.out + (size_t)row * o.n_out + n;
-          if (n + 4 <= o.n_out && ((uintptr_t)dst & 7) == 0) {
-            *reinterpret_cast<uint2*>(dst) = make_uint2(f32_to_bf16_pair(acc[t][m][4 * q], acc[t][m][4 * q + 1]),
-                                                        f32_to_bf16_pair(acc[t][m][4 * q + 2], acc[t][m][4 * q + 3]));
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (n + i < o.n_out) dst[i] = f32_to_bf16(acc[t][m][4 * q + i]);
+          for (int h = 0; h < 2; ++h) {
+            const f32x16& v = acc[t][m];
+            const auto lo = __builtin_amdgcn_permlane32_swap(f32_to_bf16_pair(v[8 * h], v[8 * h + 1]), f32_to_bf16_pair(v[8 * h + 4], v[8 * h + 5]), false, false);
+            const auto hi = __builtin_amdgcn_permlane32_swap(f32_to_bf16_pair(v[8 * h + 2], v[8 * h + 3]), f32_to_bf16_pair(v[8 * h + 6], v[8 * h + 7]), false, false);
+            *reinterpret_cast<uint4*>(mine + r * 128 + ((t * 4 + h * 2 + g) ^ (r & 7)) * 16) = make_uint4(lo[0], hi[0], lo[1], hi[1]);
           }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int lrow = i * 8 + (lane >> 3), n = n_base + (lane & 7) * 8;
+          const uint4 v = *reinterpret_cast<const uint4*>(mine + lrow * 128 + ((lane & 7) ^ (lrow & 7)) * 16);
+          if (first + lrow < row_end && n < o.n_out) *reinterpret_cast<uint4*>(o.out + (size_t)(first + lrow) * o.n_out + n) = v;
         }
+      } else if (first + r < row_end) {
+        bf16_t* dst = o.out + (size_t)(first + r) * o.n_out;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int n = n_base + t * 32 + (i / 4) * 8 + g * 4 + i % 4;
+            if (n < o.n_out) dst[n] = f32_to_bf16(acc[t][m][i]);
+          }
+      }
     }
   } else {
     const int U2 = f8_blocks(o.n_out), su2 = f8_scale_stride(o.n_out);
     float h[MT][16];
+    auto units = [&](auto code_tag) {              // (the activation is chosen once a tile)
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int lrow = (wr * MT + m) * 32 + r, row = min(row0 + lrow, row_end - 1);
-      const bool scaled = o.score != nullptr && sorted;
-      const float sc = scaled ? o.score[row] : 1.f;
-      uint32_t top = 0;
+      for (int m = 0; m < MT; ++m) {
+        const int lrow = (wr * MT + m) * 32 + r, row = min(row0 + lrow, row_end - 1);
+        const float sc = o.score != nullptr && sorted ? o.score[row] : 1.f;
+        uint32_t top = 0;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float v = exists ? bf16_to_f32(f32_to_bf16(gated_f32(act, acc[0][m][i], acc[1][m][i], sc, scaled))) : 0.f;
-        const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
-        if (b < 0x7f800000u && b > top) top = b;
-        h[m][i] = v;
+        for (int i = 0; i < 16; ++i) {
+          const float v = exists ? bf16_to_f32(f32_to_bf16(f8_unit<decltype(code_tag)::value>(act.limit, acc[0][m][i] * sc, acc[1][m][i] * sc))) : 0.f;
+          const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+          if (b < 0x7f800000u && b > top) top = b;
+          h[m][i] = v;
+        }
+        const float t2 = reduce32(__uint_as_float(top), MaxOf{});
+        if (g == 0) s_top[wc][lrow] = t2;
       }
-      const float t2 = reduce32(__uint_as_float(top), MaxOf{});
-      if (g == 0) s_top[wc][lrow] = t2;
-    }
+    };
+    if (act.code == ACT_SWISH_CLAMP) units(std::integral_constant<int, ACT_SWISH_CLAMP>{});
+    else if (act.code == ACT_GELU_TANH) units(std::integral_constant<int, ACT_GELU_TANH>{});
+    else units(std::integral_constant<int, ACT_SILU>{});
     __syncthreads();
+    // the codes through LDS, to leave as whole lines: a row's 128 are one block of the format
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const int lrow = (wr * MT + m) * 32 + r, row = row0 + lrow;
+      const int lrow = (wr * MT + m) * 32 + r;
       const float t = fmaxf(fmaxf(s_top[0][lrow], s_top[1][lrow]), fmaxf(s_top[2][lrow], s_top[3][lrow]));
       const int s = f8_scale_of(__float_as_uint(t));
       const float scale = f8_scale_value(s);
-      if (row >= row_end) continue;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         uint32_t c = f8_codes4(h[m][4 * q], h[m][4 * q + 1], h[m][4 * q + 2], h[m][4 * q + 3], scale);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if ((__float_as_uint(h[m][4 * q + i]) & 0x7f800000u) == 0x7f800000u) c |= kF8Nan << (8 * i);
-        *reinterpret_cast<uint32_t*>(o.codes + ((size_t)row * U2 + nblock) * kF8Block + wc * 32 + q * 8 + g * 4) = c;
+        *reinterpret_cast<uint32_t*>(smem + lrow * 128 + ((wc * 2 + (q >> 1)) ^ (lrow & 7)) * 16 + (q & 1) * 8 + g * 4) = c;
       }
-      if (wc == 0 && g == 0) o.scales[(size_t)row * su2 + nblock] = (uint8_t)s;
+      if (wc == 0 && g == 0 && row0 + lrow < row_end) o.scales[(size_t)(row0 + lrow) * su2 + nblock] = (uint8_t)s;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int lrow = (wid * MT + i) * 8 + (lane >> 3), row = row0 + lrow;
+      const uint4 v = *reinterpret_cast<const uint4*>(smem + lrow * 128 + ((lane & 7) ^ (lrow & 7)) * 16);
+      if (row < row_end) *reinterpret_cast<uint4*>(o.codes + ((size_t)row * U2 + nblock) * kF8Block + (lane & 7) * 16) = v;
     }
   }
+}
+
+// Blocks go to the dies round-robin; a die walks a piece of one list of (column block, row tile) of its own: column blocks four side by side, row tile by
+// row tile (siblings of an expert on end), so that what runs on a die at a time reads the same few rows and weights through its L2.
+constexpr int kSideBySide = 4;
+constexpr int kDies = 8;
+
+template <bool GATED>
+__global__ __launch_bounds__(TW* kWave, 2) void fp8_tiles_kernel(F8Tiles p, F8Out o, GatedAct act) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[kTileLds];
+  __shared__ float s_top[GATED ? TWC : 1][64 * kHighest];
+  __shared__ int s_found[3];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int slots = gridDim.x, die = blockIdx.x % kDies;
+  const int slot = die * (slots / kDies) + min(die, slots % kDies) + blockIdx.x / kDies;
+  const int c0 = slot / (kSideBySide * p.tiles) * kSideBySide, left = slot - c0 * p.tiles, wide = min(kSideBySide, p.nb - c0);
+  const int tile = left / wide, nblock = c0 + left % wide;
+  int e = 0, row0 = tile * p.height, row_end = min(p.rows, row0 + p.height);
+  if (p.offsets) {
+    // the groups' tiles are numbered through: as few of up to `height` rows as hold a group's, all of one height
+    if (threadIdx.x < kWave) {
+      int before = 0, found = -1, first_row = 0, last_row = 0;
+      for (int c = 0; c < p.groups + (p.along > 0) && found < 0; c += kWave) {
+        const int i = c + lane;
+        const int from = i < p.groups ? p.offsets[i] : p.rows, to = i < p.groups ? p.offsets[i + 1] : i == p.groups ? p.rows + p.along : p.rows;
+        const int mine = (to - from + p.height - 1) / p.height;
+        int upto = mine;
+#pragma unroll
+        for (int k = 1; k < kWave; k <<= 1) {
+          const int up = __shfl_up(upto, k, kWave);
+          if (lane >= k) upto += up;
+        }
+        const int first = before + upto - mine;
+        const unsigned long long here = __builtin_amdgcn_ballot_w64(mine > 0 && tile >= first && tile < first + mine);
+        if (here) {
+          const int l = __ffsll((long long)here) - 1;
+          const int n = __shfl(mine, l, kWave), f = __shfl(from, l, kWave), t = __shfl(to, l, kWave);
+          const int each = ((t - f + n - 1) / n + 63) & ~63;
+          found = c + l;
+          first_row = f + (tile - __shfl(first, l, kWave)) * each;
+          last_row = min(t, first_row + each);
+        }
+        before += __shfl(upto, kWave - 1, kWave);
+      }
+      if (threadIdx.x == 0) {
+        s_found[0] = found;
+        s_found[1] = first_row;
+        s_found[2] = last_row;
+      }
+    }
+    __syncthreads();
+    e = __builtin_amdgcn_readfirstlane(s_found[0]);
+    row0 = __builtin_amdgcn_readfirstlane(s_found[1]);
+    row_end = __builtin_amdgcn_readfirstlane(s_found[2]);
+    if (e < 0) return;
+  }
+  const int rows = row_end - row0;
+  if (rows <= 0) return;
+  if (rows <= 64) f8_tile<1, GATED>(p, o, act, e, row0, row_end, nblock, smem, s_top);
+  else if (rows <= 128) f8_tile<2, GATED>(p, o, act, e, row0, row_end, nblock, smem, s_top);
+  else if (rows <= 192) f8_tile<3, GATED>(p, o, act, e, row0, row_end, nblock, smem, s_top);
+  else f8_tile<4, GATED>(p, o, act, e, row0, row_end, nblock, smem, s_top);
 }
 
 bool tiles_ok(const F8Tiles& p, int x_rows) {
@@ -357,19 +399,16 @@ bool tiles_ok(const F8Tiles& p, int x_rows) {
          (!p.a_rows || (long long)x_rows * p.U * kF8Block <= 0xffffffffLL) && (long long)p.U * kF8TileBytes <= 0x7fffffffLL;
 }
 
-template <bool GATED> int launch_tiles(F8Tiles p, const F8Out& o, GatedAct act, int height, hipStream_t stream) {
+template <bool GATED> int launch_tiles(F8Tiles p, const F8Out& o, GatedAct act, hipStream_t stream) {
+  const int height = p.height;
+  if (height < 64 || height > 64 * kHighest || height % 64) return SHARPI_ERR_ARG;
   const long long tiles = p.offsets ? (long long)p.rows / height + (p.rows < p.groups ? p.rows : p.groups) + (p.along + height - 1) / height
                                     : (p.rows + height - 1) / height;
   p.nb = ceil_div(o.n_out, GATED ? kTileCols / 2 : kTileCols);
   p.tiles = (int)tiles;
   if (tiles * p.nb > 0x7fffffffLL) return SHARPI_ERR_ARG;
   const dim3 grid((unsigned)(tiles * p.nb)), block(TW * kWave);
-#define FT(MTV) fp8_tiles_kernel<MTV, GATED><<<grid, block, 0, stream>>>(p, o, act)
-  if (height == 64) FT(1);
-  else if (height == 128) FT(2);
-  else if (height == 256) FT(4);
-  else return SHARPI_ERR_ARG;
-#undef FT
+  fp8_tiles_kernel<GATED><<<grid, block, 0, stream>>>(p, o, act);
   SHARPI_CHECK_LAUNCH();
   return SHARPI_OK;
 }
@@ -377,14 +416,14 @@ template <bool GATED> int launch_tiles(F8Tiles p, const F8Out& o, GatedAct act, 
 }  // namespace
 
 // out [rows, N] bfloat16.  x: codes [x_rows, 128 U] and scales; w_rows: stored rows of one matrix; a_rows, offsets: of a sorted row list, or null; along: rows
-// behind the list's `rows`, which matrix `groups` takes (row i reads row i - rows of x if there is a_rows); height: rows of a tile (64, 128, 256).
+// behind the list's `rows`, which matrix `groups` takes (row i reads row i - rows of x if there is a_rows); height: rows of a tile at most (64, 128, 192, 256).
 SHARPI_EXPORT int sharpi_fp8_tiles(const void* x, const void* x_scales, int x_rows, const void* w_codes, const void* w_scales, int w_rows, void* out,
                                    int rows, int N, int K, const int* a_rows, const int* offsets, int groups, int along, int height, hipStream_t stream) {
   if (rows <= 0) return SHARPI_OK;
   if (N <= 0 || K <= 0 || w_rows != f8_padded_rows(N)) return SHARPI_ERR_ARG;
-  const F8Tiles p{(const uint8_t*)x, (const uint8_t*)x_scales, (const uint8_t*)w_codes, (const uint8_t*)w_scales, f8_blocks(K), w_rows, a_rows, offsets, rows, groups, (uint32_t)((long long)x_rows * f8_blocks(K) * kF8Block), along, 0, 0};
+  const F8Tiles p{(const uint8_t*)x, (const uint8_t*)x_scales, (const uint8_t*)w_codes, (const uint8_t*)w_scales, f8_blocks(K), w_rows, a_rows, offsets, rows, groups, (uint32_t)((long long)x_rows * f8_blocks(K) * kF8Block), along, height, 0, 0};
   if (!tiles_ok(p, x_rows)) return SHARPI_ERR_ARG;
-  return launch_tiles<false>(p, F8Out{(bf16_t*)out, nullptr, nullptr, nullptr, N}, GatedAct{}, height, stream);
+  return launch_tiles<false>(p, F8Out{(bf16_t*)out, nullptr, nullptr, nullptr, N}, GatedAct{}, stream);
 }
 
 // codes [rows, 128 f8_blocks(I)] and scales [rows, f8_scale_stride(I)] of act(s g) (s u); w_rows: twice I up to a multiple of 32; score [rows] or null.
@@ -394,7 +433,7 @@ SHARPI_EXPORT int sharpi_fp8_tiles_gated(const void* x, const void* x_scales, in
   if (rows <= 0) return SHARPI_OK;
   const GatedAct ga{act, limit};
   if (I <= 0 || K <= 0 || w_rows != 2 * f8_padded_rows(I) || !act_known(ga) || ((uintptr_t)codes & 15)) return SHARPI_ERR_ARG;
-  const F8Tiles p{(const uint8_t*)x, (const uint8_t*)x_scales, (const uint8_t*)w_codes, (const uint8_t*)w_scales, f8_blocks(K), w_rows, a_rows, offsets, rows, groups, (uint32_t)((long long)x_rows * f8_blocks(K) * kF8Block), along, 0, 0};
+  const F8Tiles p{(const uint8_t*)x, (const uint8_t*)x_scales, (const uint8_t*)w_codes, (const uint8_t*)w_scales, f8_blocks(K), w_rows, a_rows, offsets, rows, groups, (uint32_t)((long long)x_rows * f8_blocks(K) * kF8Block), along, height, 0, 0};
   if (!tiles_ok(p, x_rows)) return SHARPI_ERR_ARG;
-  return launch_tiles<true>(p, F8Out{nullptr, (uint8_t*)codes, (uint8_t*)scales, score, I}, ga, height, stream);
+  return launch_tiles<true>(p, F8Out{nullptr, (uint8_t*)codes, (uint8_t*)scales, score, I}, ga, stream);
 }
