@@ -76,57 +76,3 @@ __device__ __forceinline__ float f8_unit(GatedAct act, float g, float u) {
   if (act.code == ACT_GELU_TANH) return f8_unit<ACT_GELU_TANH>(act.limit, g, u);
   return f8_unit<ACT_SILU>(act.limit, g, u);
 }
-struct MaxBits {    // the larger of two magnitudes by their bits (NaN is the largest, not lost)
-  __device__ __forceinline__ float operator()(float a, float b) const {
-    const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
-    return __uint_as_float(x > y ? x : y);
-  }
-};
-
-// 32 neighbouring values of one row as they lie in memory, in lanes (row r of 16, quarter g of the block of 128): what the 16x16x128
-// instruction takes as an operand once they are codes.  f8_codes gives the codes and the block's byte; the four lanes of a row meet.
-template <typename T> struct F8Raw;
-template <> struct F8Raw<bf16_t> {
-  static constexpr int kLoads = 4, kEach = 8;
-  u32x4_t v[4];
-  __device__ __forceinline__ uint32_t top() const {
-    u16x2_t m = {0, 0};
-#pragma unroll
-    for (int i = 0; i < 16; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, v[i / 4][i % 4] & 0x7fff7fffu));
-    return (uint32_t)(m[0] > m[1] ? m[0] : m[1]) << 16;
-  }
-  __device__ __forceinline__ uint32_t top_of_finite() const {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t lo = v[i / 4][i % 4] & 0x7fffu, hi = v[i / 4][i % 4] >> 16 & 0x7fffu;
-      m = lo < 0x7f80u && lo > m ? lo : m;
-      m = hi < 0x7f80u && hi > m ? hi : m;
-    }
-    return m << 16;
-  }
-  __device__ __forceinline__ void nan_for_infinity() {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      uint32_t d = v[i / 4][i % 4];
-      if ((d & 0x7f80u) == 0x7f80u) d |= 0x7fffu;
-      if ((d & 0x7f800000u) == 0x7f800000u) d |= 0x7fff0000u;
-      v[i / 4][i % 4] = d;
-    }
-  }
-  __device__ __forceinline__ uint32_t codes(int i, float scale) const { return f8_codes4(v[i / 2][i % 2 * 2], v[i / 2][i % 2 * 2 + 1], scale); }
-};
-template <typename T> __device__ __forceinline__ i32x8 f8_codes(F8Raw<T>& raw, int& s) {
-  auto meet = [](uint32_t top) { return __float_as_uint(reduce16(reduce32(__uint_as_float(top), MaxBits{}), MaxBits{})); };
-  uint32_t top = meet(raw.top());
-  if (__builtin_amdgcn_ballot_w64(top >= 0x7f800000u)) {      // some value of the wave is not finite
-    top = meet(raw.top_of_finite());
-    raw.nan_for_infinity();
-  }
-  s = f8_scale_of(top);
-  const float scale = f8_scale_value(s);
-  i32x8 c;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = (int)raw.codes(i, scale);
-  return c;
-}

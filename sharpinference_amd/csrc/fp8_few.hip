@@ -4,8 +4,8 @@
 //   gated   h = act(s g) (s u) with (g | u) = q(x) W^T, rounded to bfloat16: the first half of a feed-forward, for one matrix or for the
 //           experts that a router picked (a block finds the rows of its expert among the picks itself)
 //   sum     out[t] = sum_j w[t, j] q(h[t, j]) W_e^T over the token's picks e (and an always-on expert): the second half, with the sum
-// q(.): rows are quantised where they are read, by the lanes that need them (32 values a lane, four lanes a block of 128): no launch and
-// no pass of its own; or they come as codes already.
+// q(.): up to 16 rows of bfloat16 are quantised by every block that reads them, into LDS (no launch and no pass of their own; the weights' first loads are on
+// their way meanwhile); other rows come as codes.
 //
 // Bound: bytes of the weights.  Each wave takes blocks of 128 of k in turn, one 4 KB unit of a tile of 32 weight rows (or half of it)
 // at a time through v_mfma_scale_f32_16x16x128: W is the A operand (rows = n), x the B operand (up to 16 rows a row block).  A lane ends
@@ -57,28 +57,66 @@ struct F8Lane {
   }
 };
 
-// A lane's 32 values of an x row for block u of k, before they are codes.
-struct F8Codes {};
-template <typename XT> struct F8Row {
-  F8Raw<XT> raw;
-  __device__ __forceinline__ void load(const void* x, const uint8_t*, size_t row, int K, int u, int g) {
-    const XT* p = (const XT*)x + row * K;
-#pragma unroll
-    for (int i = 0; i < F8Raw<XT>::kLoads; ++i) {
-      const int k = u * kF8Block + g * 32 + i * F8Raw<XT>::kEach;
-      raw.v[i] = *reinterpret_cast<const u32x4_t*>(p + min(k, K - F8Raw<XT>::kEach));
-    }
-  }
-  __device__ __forceinline__ i32x8 codes(int K, int u, int g, int& s) {
-    if (u * kF8Block + kF8Block > K) {                  // the last block of a row that ends inside of it (the same for the wave)
-#pragma unroll
-      for (int i = 0; i < F8Raw<XT>::kLoads; ++i)
-        if (u * kF8Block + g * 32 + i * F8Raw<XT>::kEach >= K) raw.v[i] = u32x4_t{0, 0, 0, 0};
-    }
-    return f8_codes(raw, s);
+// Rows' blocks of 128 as codes in LDS, in the order of the operands: block b of n rows at [b][piece][group][row][16 bytes], its bytes behind one another.
+struct F8Staged {
+  uint8_t* codes;
+  uint8_t* bytes;
+  int n;                   // rows
+  __device__ __forceinline__ i32x8 read(int b, int row, int g, int& s) const {
+    const i32x4 lo = *reinterpret_cast<const i32x4*>(codes + (((b * 2) * 4 + g) * n + row) * 16);
+    const i32x4 hi = *reinterpret_cast<const i32x4*>(codes + (((b * 2 + 1) * 4 + g) * n + row) * 16);
+    s = bytes[b * n + row];
+    return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   }
 };
-template <> struct F8Row<F8Codes> {
+// Quantises `tasks` blocks of rows of bfloat16 [.., K] into LDS, 16 lanes a block, four blocks of a lane group on their way at a time.  where(task, row, u, b, m): the
+// row of x and its block u of a task, and where it is staged (block b, row m); row < 0: nothing is read.
+template <typename F> __device__ __forceinline__ void stage_rows(const bf16_t* __restrict__ x, int K, int tasks, F8Staged to, const F& where) {
+  const int l = threadIdx.x & 15;
+  constexpr int kGroups = FW * kWave / 16, kFlight = 4;
+  for (int t0 = threadIdx.x >> 4; t0 < tasks; t0 += kGroups * kFlight) {
+    uint4 raw[kFlight];
+    int b[kFlight], m[kFlight], row[kFlight];
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+      const int t = t0 + i * kGroups;
+      int u = 0;
+      row[i] = -1;
+      if (t < tasks) where(t, row[i], u, b[i], m[i]);
+      const int k = u * kF8Block + l * 8;
+      raw[i] = row[i] >= 0 && k < K ? *reinterpret_cast<const uint4*>(x + (size_t)row[i] * K + k) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+      if (row[i] < 0) continue;                  // (16 lanes at once)
+      const uint32_t d[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      uint32_t top = 0, bad = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t lo = d[j] & 0x7fffu, hi = d[j] >> 16 & 0x7fffu;
+        top = lo < 0x7f80u && lo > top ? lo : top;
+        top = hi < 0x7f80u && hi > top ? hi : top;
+        bad |= (lo >= 0x7f80u ? 1u : 0u) << (2 * j) | (hi >= 0x7f80u ? 1u : 0u) << (2 * j + 1);
+      }
+      float t = __uint_as_float(top << 16);
+      t = fmaxf(t, row_rotated<8>(t));
+      t = fmaxf(t, row_rotated<4>(t));
+      t = fmaxf(t, row_rotated<2>(t));
+      t = fmaxf(t, row_rotated<1>(t));
+      const int s = f8_scale_of(__float_as_uint(t));
+      const float scale = f8_scale_value(s);
+      uint32_t c[2] = {f8_codes4(d[0], d[1], scale), f8_codes4(d[2], d[3], scale)};
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (bad >> j & 1) c[j / 4] = (c[j / 4] & ~(0xffu << (j % 4 * 8))) | kF8Nan << (j % 4 * 8);
+      *reinterpret_cast<uint2*>(to.codes + (((b[i] * 2 + (l >> 1 & 1)) * 4 + (l >> 2)) * to.n + m[i]) * 16 + (l & 1) * 8) = make_uint2(c[0], c[1]);
+      if (l == 0) to.bytes[b[i] * to.n + m[i]] = (uint8_t)s;
+    }
+  }
+}
+
+// A lane's 32 codes of a row's block u of k, from memory.
+struct F8Row {
   i32x4 a, b;
   int byte;
   __device__ __forceinline__ void load(const void* x, const uint8_t* scales, size_t row, int K, int u, int g) {
@@ -87,7 +125,7 @@ template <> struct F8Row<F8Codes> {
     b = *reinterpret_cast<const i32x4*>(p + 16);
     byte = scales[row * f8_scale_stride(K) + u];
   }
-  __device__ __forceinline__ i32x8 codes(int, int, int, int& s) {
+  __device__ __forceinline__ i32x8 codes(int& s) const {
     s = byte;
     return i32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   }
@@ -110,10 +148,13 @@ __device__ __forceinline__ void store_columns(bf16_t* row, int n, int columns, c
 
 // plain and gated.  R half tiles a block: of distinct columns (plain), or R / 2 of gate columns and the up columns beside them (gated).
 // n_out: columns of the result that exist; stride: of a stored row (gated: the columns from n_out to it are zeros, as their weights are).
-template <int R, int MB, typename XT, bool GATED>
-__global__ __launch_bounds__(FW* kWave, 4) void fp8_few_kernel(const void* __restrict__ x, const uint8_t* __restrict__ x_scales, F8Matrix W,
-                                                               bf16_t* __restrict__ out, int n_out, int stride, int M, int K, GatedAct act,
-                                                               F8Picks pk, int* __restrict__ clear, int n_clear) {
+// STAGED: x is bfloat16, up to 16 rows, quantised into LDS (turn: rows that fit there at a time); else codes.  A block of the plain form takes every gridDim.x-th column group.
+template <int R, int MB, bool STAGED, bool GATED>
+__global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_few_kernel(const void* __restrict__ x, const uint8_t* __restrict__ x_scales, F8Matrix W,
+                                                                            bf16_t* __restrict__ out, int n_out, int stride, int M, int K, GatedAct act,
+                                                                            F8Picks pk, int* __restrict__ clear, int n_clear, int turn, int column_groups) {
+  static_assert(!STAGED || MB == 1, "staged rows are one row block");
+  extern __shared__ __attribute__((aligned(16))) uint8_t staged_bytes[];
   constexpr int TG = GATED ? R / 2 : R;
   constexpr int RT = GATED ? R : kRound;
   __shared__ f32x4 red[FW][RT][kWave];
@@ -182,17 +223,21 @@ __global__ __launch_bounds__(FW* kWave, 4) void fp8_few_kernel(const void* __res
   const bool routed = picked && expert < pk.E;
   auto out_row = [&](int m) { return routed ? (int)members[m] : picked ? pk.T * pk.k + m : m; };
   auto x_row = [&](int m) { return routed ? members[m] / pk.k : m; };
-  const int n_base = blockIdx.x * 16 * TG;
-  F8Lane wl[R];
-#pragma unroll
-  for (int t = 0; t < R; ++t)
-    wl[t].at(W, expert, n_base / 16 + t % TG + (GATED && t >= TG ? W.rows / 32 : 0), r, g);
-  // (of a gated matrix the up rows begin at half its rows, a multiple of 32: half tile rows / 32)
-
-  for (int rb = 0; rb * 16 < rows; rb += MB) {
+  const int group_rows = STAGED ? turn : 16 * MB;
+  for (int rb = 0; rb < rows; rb += group_rows) {
+    const int here = min(rows - rb, group_rows);            // rows of this turn
+    const F8Staged st{staged_bytes, staged_bytes + W.U * kF8Block * here, here};
     size_t xr[MB];
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb) xr[mb] = x_row(min((rb + mb) * 16 + r, rows - 1));
+    for (int mb = 0; mb < MB; ++mb) xr[mb] = STAGED ? min(r, here - 1) : x_row(rb + min(mb * 16 + r, here - 1));
+    bool fresh = STAGED;                                    // (the rows are still to be staged)
+    for (int cg = blockIdx.x; cg < column_groups; cg += gridDim.x) {
+    const int n_base = cg * 16 * TG;
+    F8Lane wl[R];
+    // (of a gated matrix the up rows begin at half its rows, a multiple of 32: half tile rows / 32)
+#pragma unroll
+    for (int t = 0; t < R; ++t)
+      wl[t].at(W, expert, n_base / 16 + t % TG + (GATED && t >= TG ? W.rows / 32 : 0), r, g);
     f32x4 acc[R][MB];
 #pragma unroll
     for (int t = 0; t < R; ++t)
@@ -201,56 +246,58 @@ __global__ __launch_bounds__(FW* kWave, 4) void fp8_few_kernel(const void* __res
     struct Unit {
       i32x8 wf[R];
       int ws[R];
-      F8Row<XT> xf[MB];
+      F8Row xf[STAGED ? 1 : MB];
     };
     auto load_unit = [&](int u, Unit& un) {
 #pragma unroll
       for (int t = 0; t < R; ++t) un.wf[t] = wl[t].load(u, un.ws[t]);
+      if constexpr (!STAGED) {
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb) {
-        if (mb > 0 && (rb + mb) * 16 >= rows) continue;       // (the same for the block)
-        un.xf[mb].load(x, x_scales, xr[mb], K, u, g);
+        for (int mb = 0; mb < MB; ++mb) un.xf[mb].load(x, x_scales, xr[mb], K, u, g);     // (a row block without rows reads the last row)
       }
     };
     auto use_unit = [&](int u, Unit& un) {
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
-        if (mb > 0 && (rb + mb) * 16 >= rows) continue;
         int xs;
-        const i32x8 c = un.xf[mb].codes(K, u, g, xs);
+        const i32x8 c = STAGED ? st.read(u, (int)xr[0], g, xs) : un.xf[STAGED ? 0 : mb].codes(xs);
 #pragma unroll
         for (int t = 0; t < R; ++t) acc[t][mb] = f8_product(un.wf[t], c, acc[t][mb], un.ws[t], xs);
       }
     };
-    if constexpr (MB == 1) {
-      Unit a, b;
-      int u = w;
-      if (u < W.U) load_unit(u, a);
-      for (; u + 2 * FW < W.U; u += 2 * FW) {
-        load_unit(u + FW, b);
-        use_unit(u, a);
-        load_unit(u + 2 * FW, a);
-        use_unit(u + FW, b);
+    Unit a, b;
+    int u = w;
+    if (u < W.U) load_unit(u, a);
+    if constexpr (STAGED) {
+      if (fresh) {
+        if (rb > 0) __syncthreads();                        // (the turn before has been read)
+        stage_rows((const bf16_t*)x, K, here * W.U, st, [&](int task, int& row, int& block, int& to, int& m) {
+          m = task / W.U;
+          block = to = task - m * W.U;
+          row = x_row(rb + m);
+        });
+        __syncthreads();
+        fresh = false;
       }
-      if (u + FW < W.U) {
-        load_unit(u + FW, b);
-        use_unit(u, a);
-        use_unit(u + FW, b);
-      } else if (u < W.U) {
-        use_unit(u, a);
-      }
-    } else {
-      for (int u = w; u < W.U; u += FW) {
-        Unit a;
-        load_unit(u, a);
-        use_unit(u, a);
-      }
+    }
+    for (; u + 2 * FW < W.U; u += 2 * FW) {
+      load_unit(u + FW, b);
+      use_unit(u, a);
+      load_unit(u + 2 * FW, a);
+      use_unit(u + FW, b);
+    }
+    if (u + FW < W.U) {
+      load_unit(u + FW, b);
+      use_unit(u, a);
+      use_unit(u + FW, b);
+    } else if (u < W.U) {
+      use_unit(u, a);
     }
 
     if constexpr (GATED) {
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
-        if (mb > 0 && (rb + mb) * 16 >= rows) continue;
+        if (mb > 0 && mb * 16 >= here) continue;
         __syncthreads();
 #pragma unroll
         for (int t = 0; t < R; ++t) red[w][t][lane] = acc[t][mb];
@@ -262,9 +309,9 @@ __global__ __launch_bounds__(FW* kWave, 4) void fp8_few_kernel(const void* __res
             gv += red[ww][w][lane];
             uv += red[ww][w + TG][lane];
           }
-          const int m = (rb + mb) * 16 + r, n = n_base + w * 16 + g * 4;
-          if (m < rows && n < stride) {
-            const int orow = out_row(m);
+          const int m = mb * 16 + r, n = n_base + w * 16 + g * 4;
+          if (m < here && n < stride) {
+            const int orow = out_row(rb + m);
             const bool scaled = routed && pk.w != nullptr;
             const float sc = scaled ? pk.w[orow] : 1.0f;
             f32x4 o;
@@ -279,7 +326,7 @@ __global__ __launch_bounds__(FW* kWave, 4) void fp8_few_kernel(const void* __res
       for (int p0 = 0; p0 < R * MB; p0 += kRound) {
         bool any = false;
 #pragma unroll
-        for (int p = 0; p < kRound; ++p) any = any || (p0 + p < R * MB && (rb + (p0 + p) % MB) * 16 < rows);
+        for (int p = 0; p < kRound; ++p) any = any || (p0 + p < R * MB && (p0 + p) % MB * 16 < here);
         if (!any) continue;
         __syncthreads();
 #pragma unroll
@@ -291,20 +338,24 @@ __global__ __launch_bounds__(FW* kWave, 4) void fp8_few_kernel(const void* __res
           f32x4 v = red[0][w][lane];
 #pragma unroll
           for (int ww = 1; ww < FW; ++ww) v += red[ww][w][lane];
-          const int m = (rb + mb) * 16 + r, n = n_base + t * 16 + g * 4;
-          if (m < rows && n < n_out) store_columns(out + (size_t)m * stride, n, n_out, v);
+          const int m = mb * 16 + r, n = n_base + t * 16 + g * 4;
+          if (m < here && n < n_out) store_columns(out + (size_t)(rb + m) * stride, n, n_out, v);
         }
       }
+    }
     }
   }
 }
 
 // The sum over a token's picks.  R half tiles of columns a block, MB row blocks of tokens; blockIdx.y: the share of the blocks of k.
 // part [S][tiles][MB][R][64 lanes] float4, counters [tiles] zero before the launch (both unused if S is 1).
-template <int R, int MB, typename XT>
-__global__ __launch_bounds__(FW* kWave, 4) void fp8_sum_kernel(const void* __restrict__ h, const uint8_t* __restrict__ h_scales, F8Matrix W,
-                                                               bf16_t* __restrict__ out, int n_out, int K, F8Picks pk, int weighted,
-                                                               f32x4* __restrict__ part, int* __restrict__ counters) {
+// STAGED: h is bfloat16, up to 16 tokens, quantised into LDS `chunk` blocks of k (a multiple of 2 FW) at a time; else codes.
+template <int R, int MB, bool STAGED>
+__global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_sum_kernel(const void* __restrict__ h, const uint8_t* __restrict__ h_scales, F8Matrix W,
+                                                                            bf16_t* __restrict__ out, int n_out, int K, F8Picks pk, int weighted,
+                                                                            f32x4* __restrict__ part, int* __restrict__ counters, int chunk) {
+  static_assert(!STAGED || MB == 1, "staged rows are one row block");
+  extern __shared__ __attribute__((aligned(16))) uint8_t staged_bytes[];
   __shared__ f32x4 red[FW][kRound][kWave];
   __shared__ int ids[kFewPairs];
   __shared__ float wts[kFewPairs];
@@ -356,56 +407,55 @@ __global__ __launch_bounds__(FW* kWave, 4) void fp8_sum_kernel(const void* __res
   for (int t = 0; t < R; ++t)
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) total[t][mb] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // the row of h that a token has for an entry (-1: none) and its weight
+  auto row_of = [&](int code, int tok, float& weight) {
+    weight = 1.f;
+    if (tok >= pk.T) return -1;
+    if (!pk.ids) return tok;
+    const int e = code & 0xffff, occurrence = code >> 16;
+    if (e == pk.E) return n_pairs + tok;
+    int row = -1, seen = 0;
+    for (int j = 0; j < pk.k; ++j) {
+      const int p = tok * pk.k + j;
+      if (ids[p] == e) {
+        if (seen == occurrence) {
+          row = p;
+          if (weighted) weight = wts[p];
+        }
+        ++seen;
+      }
+    }
+    return row;
+  };
+  auto code_of = [&](int at) { return pk.ids ? entry[at] : 0; };
   struct Unit {
     i32x8 wf[R];
-    int ws[R], u;
-    F8Row<XT> xf[MB];
+    int ws[R];
+    F8Row xf[STAGED ? 1 : MB];
     float weight[MB];
     int row[MB];
   };
   auto load_unit = [&](int i, Unit& un) {
-    const int at = i / W.U;
-    un.u = i - at * W.U;
-    const int code = pk.ids ? __builtin_amdgcn_readfirstlane(entry[at]) : 0;
-    const int e = code & 0xffff, occurrence = code >> 16;
+    i = min(i, end - 1);                            // (past the share: its last block once more, for nobody)
+    const int at = i / W.U, u = i - at * W.U, code = __builtin_amdgcn_readfirstlane(code_of(at));
 #pragma unroll
     for (int t = 0; t < R; ++t) {
       F8Lane wl;
-      wl.at(W, e, n_base / 16 + t, r, g);
-      un.wf[t] = wl.load(un.u, un.ws[t]);
+      wl.at(W, code & 0xffff, n_base / 16 + t, r, g);
+      un.wf[t] = wl.load(u, un.ws[t]);
     }
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
-      const int tok = mb * 16 + r;
-      int row = -1;
-      float weight = 1.f;
-      if (tok < pk.T) {
-        if (!pk.ids) row = tok;
-        else if (e == pk.E) row = n_pairs + tok;
-        else {
-          int seen = 0;
-          for (int j = 0; j < pk.k; ++j) {
-            const int p = tok * pk.k + j;
-            if (ids[p] == e) {
-              if (seen == occurrence) {
-                row = p;
-                if (weighted) weight = wts[p];
-              }
-              ++seen;
-            }
-          }
-        }
-      }
-      un.row[mb] = row;
-      un.weight[mb] = weight;
-      un.xf[mb].load(h, h_scales, row < 0 ? 0 : row, K, un.u, g);      // (row 0: read for a token without this expert, never added)
+      un.row[mb] = row_of(code, mb * 16 + r, un.weight[mb]);
+      if constexpr (!STAGED) un.xf[mb].load(h, h_scales, max(un.row[mb], 0), K, u, g);      // (row 0: read for a token without this expert, never added)
     }
   };
-  auto use_unit = [&](Unit& un) {
+  const F8Staged st{staged_bytes, staged_bytes + chunk * kF8Block * pk.T, pk.T};
+  auto use_unit = [&](int staged_block, Unit& un) {
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
       int xs;
-      const i32x8 c = un.xf[mb].codes(K, un.u, g, xs);
+      const i32x8 c = STAGED ? st.read(staged_block, min(r, pk.T - 1), g, xs) : un.xf[STAGED ? 0 : mb].codes(xs);
 #pragma unroll
       for (int t = 0; t < R; ++t) {
         const f32x4 v = f8_product(un.wf[t], c, f32x4{0.f, 0.f, 0.f, 0.f}, un.ws[t], xs);
@@ -414,28 +464,32 @@ __global__ __launch_bounds__(FW* kWave, 4) void fp8_sum_kernel(const void* __res
       }
     }
   };
-  if constexpr (MB == 1) {
+  if (first < end) {
     Unit a, b;
-    int i = first + w;
-    if (i < end) load_unit(i, a);
-    for (; i + 2 * FW < end; i += 2 * FW) {
-      load_unit(i + FW, b);
-      use_unit(a);
-      load_unit(i + 2 * FW, a);
-      use_unit(b);
-    }
-    if (i + FW < end) {
-      load_unit(i + FW, b);
-      use_unit(a);
-      use_unit(b);
-    } else if (i < end) {
-      use_unit(a);
-    }
-  } else {
-    for (int i = first + w; i < end; i += FW) {
-      Unit a;
-      load_unit(i, a);
-      use_unit(a);
+    load_unit(first + w, a);
+    for (int c0 = first; c0 < end; c0 += chunk) {
+      if constexpr (STAGED) {
+        if (c0 > first) __syncthreads();            // (the chunk before has been read)
+        const int blocks = min(chunk, end - c0);
+        stage_rows((const bf16_t*)h, K, blocks * pk.T, st, [&](int task, int& row, int& block, int& to, int& m) {
+          to = task / pk.T;
+          m = task - to * pk.T;
+          const int at = (c0 + to) / W.U;
+          float weight;
+          block = c0 + to - at * W.U;
+          row = row_of(code_of(at), m, weight);
+        });
+        __syncthreads();
+      }
+      for (int j = w; j < chunk; j += 2 * FW) {
+        const int i = c0 + j;
+        if (i >= end) break;
+        load_unit(i + FW, b);
+        use_unit(j, a);
+        if (i + FW >= end) break;
+        load_unit(i + 2 * FW, a);
+        use_unit(j + FW, b);
+      }
     }
   }
 
@@ -483,10 +537,12 @@ __global__ __launch_bounds__(FW* kWave, 4) void fp8_sum_kernel(const void* __res
 
 // x operand of a call: codes, or (up to 16 rows) bfloat16 whose runs of eight lie at 16-byte addresses
 enum : int { X_BF16 = DT_BF16, X_CODES = 2 };
+constexpr int kStagedMost = 48 * 1024;          // bytes of LDS for staged rows
 bool rows_ok(const void* x, int kind, int M, int K) {
   if (((uintptr_t)x & 15) != 0) return false;
   return kind == X_CODES || (kind == X_BF16 && K % 8 == 0 && M <= 16);
 }
+int staged_size(int rows, int blocks) { return rows * blocks * (kF8Block + 1) + 16; }
 bool matrix_ok(const F8Matrix& W, long long matrices) {
   return W.rows > 0 && W.rows % kF8Tile == 0 && W.U > 0 && matrices > 0 && (long long)W.rows * W.U < 0x7fffffffLL;
 }
@@ -499,23 +555,23 @@ SHARPI_EXPORT int sharpi_fp8_few(const void* x, const void* x_scales, int kind, 
   if (M <= 0) return SHARPI_OK;
   const F8Matrix W{(const uint8_t*)w_codes, (const uint8_t*)w_scales, w_rows, f8_blocks(K)};
   if (M > kFewRows || N <= 0 || K <= 0 || w_rows != f8_padded_rows(N) || !matrix_ok(W, 1) || !rows_ok(x, kind, M, K)) return SHARPI_ERR_ARG;
-  const int mb = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-  const dim3 grid((unsigned)ceil_div(N, 16 * R)), block(FW * kWave);
-#define FF(RV, MBV, XT) \
-  fp8_few_kernel<RV, MBV, XT, false><<<grid, block, 0, stream>>>(x, (const uint8_t*)x_scales, W, (bf16_t*)out, N, N, M, K, GatedAct{}, F8Picks{}, nullptr, 0)
-#define FF_MB(RV, XT)        \
-  if (mb == 1) FF(RV, 1, XT); \
-  else if (mb == 2) FF(RV, 2, XT); \
-  else FF(RV, 4, XT)
-#define FF_X(RV)                                          \
-  if (kind == X_CODES) { FF_MB(RV, F8Codes); }            \
-  else if (mb == 1) FF(RV, 1, bf16_t);                    \
-  else return SHARPI_ERR_ARG
+  const int mb = M <= 16 ? 1 : M <= 32 ? 2 : 4, groups = ceil_div(N, 16 * R);
+  const int lds = kind == X_CODES ? 0 : staged_size(M, W.U);
+  if (lds > kStagedMost) return SHARPI_ERR_ARG;
+  // (as many blocks as stay at once: each stages the rows for all its column groups)
+  const int most = lds ? 4 * compute_units() : groups;
+  const dim3 grid((unsigned)(groups < most ? groups : most)), block(FW * kWave);
+#define FF(RV, MBV, STG) \
+  fp8_few_kernel<RV, MBV, STG, false><<<grid, block, lds, stream>>>(x, (const uint8_t*)x_scales, W, (bf16_t*)out, N, N, M, K, GatedAct{}, F8Picks{}, nullptr, 0, M, groups)
+#define FF_X(RV)                          \
+  if (kind != X_CODES) FF(RV, 1, true);   \
+  else if (mb == 1) FF(RV, 1, false);     \
+  else if (mb == 2) FF(RV, 2, false);     \
+  else FF(RV, 4, false)
   if (R == 1) { FF_X(1); }
   else if (R == 2) { FF_X(2); }
   else return SHARPI_ERR_ARG;
 #undef FF_X
-#undef FF_MB
 #undef FF
   SHARPI_CHECK_LAUNCH();
   return SHARPI_OK;
@@ -540,22 +596,21 @@ SHARPI_EXPORT int sharpi_fp8_few_gated(const void* x, const void* x_scales, int 
   if (I <= 0 || K <= 0 || w_rows != 2 * f8_padded_rows(I) || stride != (I + 7) / 8 * 8 || !act_known(ga) || !picks_ok(pk) ||
       !matrix_ok(W, E + pk.shared) || !rows_ok(x, kind, T, K) || ((uintptr_t)h & 15)) return SHARPI_ERR_ARG;
   const int mb = T <= 16 ? 1 : T <= 32 ? 2 : 4;
-  const int groups = ids ? (T * k < E ? T * k : E) + pk.shared : 1;
-  const dim3 grid((unsigned)ceil_div(I, 8 * R), (unsigned)groups), block(FW * kWave);
-#define FG(RV, MBV, XT) \
-  fp8_few_kernel<RV, MBV, XT, true><<<grid, block, 0, stream>>>(x, (const uint8_t*)x_scales, W, (bf16_t*)h, I, stride, T, K, ga, pk, clear, n_clear)
-#define FG_MB(RV, XT)        \
-  if (mb == 1) FG(RV, 1, XT); \
-  else if (mb == 2) FG(RV, 2, XT); \
-  else FG(RV, 4, XT)
-#define FG_X(RV)                                          \
-  if (kind == X_CODES) { FG_MB(RV, F8Codes); }            \
-  else if (mb == 1) FG(RV, 1, bf16_t);                    \
-  else return SHARPI_ERR_ARG
+  const int groups = ids ? (T * k < E ? T * k : E) + pk.shared : 1, column_groups = ceil_div(I, 8 * R);
+  const int lds = kind == X_CODES ? 0 : staged_size(T, W.U);       // (rows of a turn: the tokens')
+  if (lds > kStagedMost) return SHARPI_ERR_ARG;
+  const dim3 grid((unsigned)column_groups, (unsigned)groups), block(FW * kWave);
+#define FG(RV, MBV, STG) \
+  fp8_few_kernel<RV, MBV, STG, true><<<grid, block, lds, stream>>>(x, (const uint8_t*)x_scales, W, (bf16_t*)h, I, stride, T, K, ga, pk, clear, n_clear, T, column_groups)
+#define FG_X(RV)                          \
+  if (kind != X_CODES) FG(RV, 1, true);   \
+  else if (mb == 1) FG(RV, 1, false);     \
+  else if (mb == 2) FG(RV, 2, false);     \
+  else FG(RV, 4, false)
   if (R == 2) { FG_X(2); }
+  else if (R == 4) { FG_X(4); }
   else return SHARPI_ERR_ARG;
 #undef FG_X
-#undef FG_MB
 #undef FG
   SHARPI_CHECK_LAUNCH();
   return SHARPI_OK;
@@ -572,13 +627,17 @@ SHARPI_EXPORT int sharpi_fp8_few_sum(const void* h, const void* h_scales, int ki
       (S > 1 && (!part || !counters)) || (long long)(kFewPairs + 1) * W.U > 0x7fffffffLL) return SHARPI_ERR_ARG;
   const int mb = T <= 16 ? 1 : T <= 32 ? 2 : 4;
   const dim3 grid((unsigned)ceil_div(N, 16 * R), (unsigned)S), block(FW * kWave);
-#define FS(RV, MBV, XT) \
-  fp8_sum_kernel<RV, MBV, XT><<<grid, block, 0, stream>>>(h, (const uint8_t*)h_scales, W, (bf16_t*)out, N, K, pk, wts != nullptr, (f32x4*)part, counters)
-#define FS_MB(RV)            \
-  if (kind != X_CODES) FS(RV, 1, bf16_t); \
-  else if (mb == 1) FS(RV, 1, F8Codes); \
-  else if (mb == 2) FS(RV, 2, F8Codes); \
-  else FS(RV, 4, F8Codes)
+  // blocks of k staged at a time: up to 32 KB of rows
+  const int chunk = T <= 8 ? 4 * FW : 2 * FW;
+  const int lds = kind == X_CODES ? 0 : staged_size(T, chunk);
+#define FS(RV, MBV, STG) \
+  fp8_sum_kernel<RV, MBV, STG><<<grid, block, lds, stream>>>(h, (const uint8_t*)h_scales, W, (bf16_t*)out, N, K, pk, wts != nullptr, (f32x4*)part, counters, \
+                                                             STG ? chunk : 0x40000000)
+#define FS_MB(RV)                       \
+  if (kind != X_CODES) FS(RV, 1, true); \
+  else if (mb == 1) FS(RV, 1, false);   \
+  else if (mb == 2) FS(RV, 2, false);   \
+  else FS(RV, 4, false)
   if (R == 1) { FS_MB(1); }
   else if (R == 2) { FS_MB(2); }
   else return SHARPI_ERR_ARG;

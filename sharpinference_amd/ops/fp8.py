@@ -21,6 +21,7 @@ FP8_TILE = 32                  # weight rows of a stored tile
 FP8_FEW_ROWS = 64              # rows of the weight-streaming kernels (csrc/fp8_few.hip kFewRows)
 FP8_FEW_PAIRS = 1024           # (token, pick) pairs of the same (kFewPairs)
 FP8_MAX_EXPERTS = 1023         # experts of a layer, one more may be always on (kFewExperts, kMaxGroups)
+FP8_STAGED_BYTES = 48 * 1024   # LDS for rows that are quantised where they are read (kStagedMost)
 _X_CODES = 2                   # csrc/fp8_few.hip X_CODES
 
 
@@ -188,10 +189,12 @@ def _rows_of(x) -> Fp8Rows:
 
 
 def _few_rows_of(x):
-    """(tensor, scales, kind) of the rows as the weight-streaming kernels take them: up to 16 rows of bfloat16 are quantised where they are read."""
+    """(tensor, scales, kind) of the rows as the weight-streaming kernels take them: up to 16 rows of bfloat16 are quantised where they are read, if they
+    fit in LDS."""
     if isinstance(x, Fp8Rows):
         return x.codes, x.scales, _X_CODES
-    if x.dtype == torch.bfloat16 and x.shape[0] <= 16 and x.shape[1] % 8 == 0 and x.data_ptr() % 16 == 0:
+    if (x.dtype == torch.bfloat16 and x.shape[0] <= 16 and x.shape[1] % 8 == 0 and x.data_ptr() % 16 == 0
+            and x.shape[0] * _blocks(x.shape[1]) * (FP8_BLOCK + 1) + 16 <= FP8_STAGED_BYTES):
         return x, None, _code(x.dtype)
     q = quantize_rows(x)
     return q.codes, q.scales, _X_CODES
