@@ -511,20 +511,22 @@ __global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_sum_kernel(cons
 #pragma unroll
       for (int ww = 1; ww < FW; ++ww) v += red[ww][w][lane];
       if (S == 1) store((p0 + w) / MB, (p0 + w) % MB, v);
-      else part[share * share_parts + blockIdx.x * tile_parts + (size_t)(p0 + w) * kWave + lane] = v;
+      else {
+        float* dst = reinterpret_cast<float*>(part + share * share_parts + blockIdx.x * tile_parts + (size_t)(p0 + w) * kWave + lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) __hip_atomic_store(dst + i, v[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
     }
   }
   if (S == 1) return;
-  // what the block wrote is everyone's before its ticket counts; who draws the last ticket adds the shares up in their order
-  __threadfence();
+  // What the block wrote is in memory before its ticket counts; who draws the last ticket adds the shares up in their order.  The shares are written and
+  // read as words that all dies see (agent scope), so a wait for the wave's own stores is all that the ticket needs: a fence writes back the
+  // whole L2 of the die, every wave anew (84 MB of weights in 480 blocks: 160 us).
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  if (threadIdx.x == 0) {
-    const int before = __hip_atomic_fetch_add(&counters[blockIdx.x], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-    is_last = before == S - 1;
-  }
+  if (threadIdx.x == 0) is_last = __hip_atomic_fetch_add(&counters[blockIdx.x], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == S - 1;
   __syncthreads();
   if (!is_last) return;
-  __threadfence();
   for (int p = w; p < R * MB; p += FW) {
     const float* src = reinterpret_cast<const float*>(part + blockIdx.x * tile_parts + (size_t)p * kWave + lane);
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
