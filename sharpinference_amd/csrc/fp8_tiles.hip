@@ -14,7 +14,7 @@ namespace {
 
 constexpr int TW = 8;                  // waves a block: 2 along the rows x 4 along the columns
 constexpr int TWC = 4;
-constexpr int kTileCols = 256;         // weight rows of a block: 64 a column wave, two tiles of 32
+constexpr int columns_of(int nt) { return 32 * nt * TWC; }      // weight rows of a block: nt tiles of 32 a column wave
 constexpr int kMaxGroups = 1024;
 
 struct F8Tiles {
@@ -45,23 +45,29 @@ struct F8Out {
 // of the banks.
 __device__ __forceinline__ int row_piece(int row, int piece) { return piece ^ ((row >> 2) & 3); }
 
-// LDS holds a ring of slots, a slot one step (64 of k: 16 KB of weights, 4 KB of rows for each MT) of tall tiles, or two steps of tiles of up to 128 rows,
+// Two kernels.  PAIRED: tiles of up to 128 rows, two blocks a compute unit, which fill each other's gaps (a tile's first loads, its barriers, its
+// end); the other: tiles of up to 256, one block a unit, for what many rows share.
+// LDS holds a ring of slots, a slot one step (64 of k: 16 KB of weights, 4 KB of rows for each MT), or two steps of low tiles in a block of its own,
 // whose steps are short beside a barrier.
-constexpr int slot_steps(int mt) { return mt <= 2 ? 2 : 1; }
-constexpr int slots(int mt) { return mt <= 2 ? 3 : 4; }
-constexpr int kWStep = 16384;
-constexpr int step_bytes(int mt) { return kWStep + 4096 * mt; }
-constexpr int scales_at(int mt) { return slots(mt) * slot_steps(mt) * step_bytes(mt); }
-constexpr int kTileLds = scales_at(2) + 3 * 2048;
-static_assert(scales_at(4) <= scales_at(2) && scales_at(3) <= scales_at(2) && scales_at(1) <= scales_at(2), "the largest ring");
-constexpr int kHighest = 4;            // a tile has up to 64 x this many rows
+constexpr int step_bytes(int mt, int nt) { return 8192 * nt + 4096 * mt; }
+template <bool PAIRED> struct Ring {
+  static constexpr int kHighest = PAIRED ? 2 : 4;                       // a tile has up to 64 x this many rows
+  static constexpr int steps(int mt) { return !PAIRED && mt <= 2 ? 2 : 1; }
+  static constexpr int slots(int mt) { return PAIRED || mt <= 2 ? 3 : 4; }
+  static constexpr int scales_at(int mt) { return slots(mt) * steps(mt) * step_bytes(mt, 2); }
+  static constexpr int kRowScales = 256 * kHighest, kChunk = kRowScales + 1024;       // bytes of a chunk's scales: rows', then weights'
+  static constexpr int kLds = scales_at(2) + 3 * kChunk;
+  static_assert(scales_at(1) <= scales_at(2) && (PAIRED || (scales_at(3) <= scales_at(2) && scales_at(4) <= scales_at(2))), "the largest ring");
+};
 
-// One tile: rows row0 .. row_end (up to 64 MT of them) of matrix e against column block nblock.  MT: groups of 32 rows a wave.
-template <int MT, bool GATED>
+// One tile: rows row0 .. row_end (up to 64 MT of them) of matrix e against column block nblock.  MT: groups of 32 rows a wave; NT: weight tiles of a wave.
+template <int MT, int NT, bool GATED, bool PAIRED>
 __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedAct act, int e, int row0, int row_end, int nblock, unsigned char* smem,
-                                        float (*s_top)[64 * kHighest]) {
-  constexpr int NS = slot_steps(MT), RING = slots(MT) * NS, AHEAD = RING - NS;      // (steps)
-  constexpr int kStep = step_bytes(MT), kSAt = scales_at(MT);
+                                        float (*s_top)[64 * Ring<PAIRED>::kHighest]) {
+  using RG = Ring<PAIRED>;
+  constexpr int NS = RG::steps(MT), RING = RG::slots(MT) * NS, AHEAD = RING - NS;      // (steps)
+  static_assert(NT == 2 || !GATED, "a gated tile's columns are a block of the format");
+  constexpr int kTileCols = columns_of(NT), kWStep = 8192 * NT, kStep = step_bytes(MT, NT), kSAt = RG::scales_at(MT);
   const int lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 31, g = lane >> 5;
   const int wr = wid / TWC, wc = wid % TWC;
@@ -70,7 +76,7 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
   const int half = p.w_rows / 64;                // gated: tiles of the gate rows
   const bool exists = !GATED || nblock * (kTileCols / 64) + wc < half;
   // Loads go straight into LDS.  Weights: wave wid brings tile wid of the block's eight (gated: a wave column's gate tile, then its up tile), a step is
-  // 2 KB of it on end.  Rows: a load brings 16 rows of 64 bytes, their 16-byte pieces exchanged by row bits (row_piece).  Rows behind the last read it
+  // 2 KB of it on end; of four tiles half a step each.  Rows: a load brings 16 rows of 64 bytes, their 16-byte pieces exchanged by row bits (row_piece).  Rows behind the last read it
   // again; what they give is never stored.  Scales: a chunk of four blocks of k is a word a row; waves 0 to 3 bring those of 64 rows each,
   // waves 4 to 7 those of two weight tiles each.
   auto block_tile = [&](int lt) {
@@ -78,7 +84,7 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
     else return min(nblock * (kTileCols / 32) + lt, p.w_rows / 32 - 1);
   };
   const size_t w_at = (size_t)e * (p.w_rows / 32);
-  const u32x4 wb = buffer_of(p.w + (w_at + block_tile(wid)) * p.U * kF8TileBytes, (uint32_t)p.U * kF8TileBytes);
+  const u32x4 wb = buffer_of(p.w + (w_at + block_tile(NT == 2 ? wid : wid >> 1)) * p.U * kF8TileBytes, (uint32_t)p.U * kF8TileBytes);
   const uint32_t lds0 = lds_address((const char*)smem);
   const uint32_t x_stride = (uint32_t)p.U * kF8Block;
   const size_t x_first = p.a_rows ? 0 : row0;             // (rows in a row: the tile's own piece of x, at any distance)
@@ -90,9 +96,11 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
   };
   constexpr int XL = (MT + 1) / 2;                        // loads of rows a wave and step (of 4 MT; some twice, to the same place)
   const int steps = 2 * p.U;
-  const uint32_t w_off[2] = {(uint32_t)lane * 16, (uint32_t)lane * 16 + 1024};
+  const uint32_t w_off[2] = {(uint32_t)lane * 16 + (NT == 1 ? (wid & 1) * 1024 : 0), (uint32_t)lane * 16 + 1024};
   auto load_w = [&](int s, uint32_t at) {                 // (past the end: the last step once more, for nobody)
-    load_two_to_lds<false>(wb, w_off[0], w_off[1], min(s, steps - 1) * 2048, lds0 + at + wid * 2048, lds0 + at + wid * 2048 + 1024);
+    const uint32_t from = min(s, steps - 1) * 2048, to = lds0 + at + wid * (1024 * NT);
+    if constexpr (NT == 2) load_two_to_lds<false>(wb, w_off[0], w_off[1], from, to, to + 1024);
+    else load_to_lds<false>(wb, w_off[0], from, to);
   };
   uint32_t x_off[XL], xs_off;
   int x_to[XL];
@@ -109,7 +117,7 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
     xs_off = (uint32_t)x_row(lrow) * (U4 * 4);
     sb = buffer_of(p.xs + x_first * (U4 * 4), p.a_rows ? (uint32_t)(p.x_bytes / x_stride) * (U4 * 4) : (uint32_t)(row_end - row0) * (U4 * 4));
   } else {
-    const int lt = (wid - 4) * 2;
+    const int lt = (wid - 4) * 2 % (4 * NT);              // (of four tiles twice, to the same place)
     const int t0 = block_tile(lt), t1 = block_tile(lt + 1);
     const uint8_t* base = p.ws + w_at * U4 * 128;
     const int low = min(t0, t1);                          // (the descriptor begins at the lower of the two tiles)
@@ -118,14 +126,14 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) sb[i] = (uint32_t)__builtin_amdgcn_readfirstlane(sb[i]);
-  const uint32_t s_lds = lds0 + kSAt + (wid < 4 ? min(wid, MT - 1) * 256 : 1024 + (wid - 4) * 256);
+  const uint32_t s_lds = lds0 + kSAt + (wid < 4 ? min(wid, MT - 1) * 256 : RG::kRowScales + (wid - 4) % (2 * NT) * 256);
   const uint32_t s_step = wid < 4 ? 4 : 128;
   // waited for here: the compiler's own waits must not fall among the loads below, which it does not know of
 #pragma unroll
   for (int i = 0; i < XL; ++i) asm volatile("" : "+v"(x_off[i]));
   asm volatile("" : "+v"(xs_off));
   // the scales of the chunk behind chunk c, once a chunk; the other blocks' loads go where nobody reads
-  auto load_s = [&](int c, bool first) { load_words_to_lds(sb, xs_off, min(c + 1, U4 - 1) * s_step, s_lds + (first ? ((c + 1) & 1) * 2048 : 4096)); };
+  auto load_s = [&](int c, bool first) { load_words_to_lds(sb, xs_off, min(c + 1, U4 - 1) * s_step, s_lds + (first ? ((c + 1) & 1) : 2) * RG::kChunk); };
   auto load_x = [&](int s, uint32_t at) {
     uint32_t to[XL];
 #pragma unroll
@@ -139,37 +147,37 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
     load_x(s, s * kStep);
   }
 
-  f32x16 acc[2][MT];
+  f32x16 acc[NT][MT];
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[t][m][i] = 0.f;
   // operand addresses: W of the step, and piece q of a lane's 32 bytes of its rows
-  int w_lds = wc * 4096 + lane * 16, x_lds[2];
+  int w_lds = wc * (2048 * NT) + lane * 16, x_lds[2];
 #pragma unroll
   for (int q = 0; q < 2; ++q) x_lds[q] = kWStep + (wr * MT * 32 + r) * 64 + row_piece(r, g * 2 + q) * 16;
-  const int ws_lds = kSAt + 1024 + wc * 256 + r * 4, xs_lds = kSAt + (wr * MT * 32 + r) * 4;
+  const int ws_lds = kSAt + RG::kRowScales + wc * (128 * NT) + r * 4, xs_lds = kSAt + (wr * MT * 32 + r) * 4;
   constexpr int H0 = (MT + 1) / 2, H1 = MT / 2;
-  i32x8 wf[2], x0[H0], x1[H1 > 0 ? H1 : 1];
-  int bw[2], bx[MT];                               // the block's scales
+  i32x8 wf[NT], x0[H0], x1[H1 > 0 ? H1 : 1];
+  int bw[NT], bx[MT];                               // the block's scales
   auto operand = [&](int a, int b) {
     const i32x4 lo = *reinterpret_cast<const i32x4*>(smem + a), hi = *reinterpret_cast<const i32x4*>(smem + b);
     return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
-  auto read_w = [&](i32x8 (&to)[2]) {
+  auto read_w = [&](i32x8 (&to)[NT]) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) to[t] = operand(w_lds + t * 2048, w_lds + t * 2048 + 1024);
+    for (int t = 0; t < NT; ++t) to[t] = operand(w_lds + t * 2048, w_lds + t * 2048 + 1024);
   };
   auto read_rows = [&](i32x8* to, int m0, int n) {
 #pragma unroll
     for (int m = 0; m < n; ++m) to[m] = operand(x_lds[0] + (m0 + m) * 2048, x_lds[1] + (m0 + m) * 2048);
   };
-  auto read_scales = [&](int u, int (&w)[2], int (&x)[MT]) {
-    const int at = (u & 3) + (u >> 2 & 1) * 2048;
+  auto read_scales = [&](int u, int (&w)[NT], int (&x)[MT]) {
+    const int at = (u & 3) + (u >> 2 & 1) * RG::kChunk;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) w[t] = smem[ws_lds + t * 128 + at];
+    for (int t = 0; t < NT; ++t) w[t] = smem[ws_lds + t * 128 + at];
 #pragma unroll
     for (int m = 0; m < MT; ++m) x[m] = smem[xs_lds + m * 128 + at];
   };
@@ -186,7 +194,7 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
     constexpr int hh = decltype(half_tag)::value;
     auto row_products = [&](const i32x8& rows, int m) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) acc[t][m] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[t], rows, acc[t][m], 0, 0, 0, bw[t], 0, bx[m]);
+      for (int t = 0; t < NT; ++t) acc[t][m] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[t], rows, acc[t][m], 0, 0, 0, bw[t], 0, bx[m]);
     };
     if constexpr (H1 > 0) read_rows(x1, H0, H1);
     row_products(x0[0], 0);
@@ -199,7 +207,7 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
     __builtin_amdgcn_sched_barrier(0);             // products of the first row groups stay ahead of the barrier, those of the others behind it
     if constexpr (NS == 1 || hh == 1) {
       // the next slot is here, and everyone has read the one before: counted are the slots behind it (a scales' load among them makes the wait one longer)
-      lds_loads_wait<NS == 1 ? 2 * (2 + XL) : 2 * (2 + XL)>();
+      lds_loads_wait<(AHEAD - NS) * (NT + XL)>();
       __syncthreads();
     }
     const int turn = at == (RING - 1) * kStep ? (1 - RING) * kStep : kStep;
@@ -208,8 +216,8 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
     x_lds[0] += turn;
     x_lds[1] += turn;
     __builtin_amdgcn_sched_barrier(0);
-    i32x8 wn[2];
-    int nw[2], nx[MT];
+    i32x8 wn[NT];
+    int nw[NT], nx[MT];
     if constexpr (hh == 1) read_scales((s + 1) >> 1, nw, nx);
     read_w(wn);
     read_rows(x0, 0, H0);
@@ -220,10 +228,10 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
 #pragma unroll
     for (int m = 1; m < H1; ++m) row_products(x1[m], H0 + m);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) wf[t] = wn[t];
+    for (int t = 0; t < NT; ++t) wf[t] = wn[t];
     if constexpr (hh == 1) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) bw[t] = nw[t];
+      for (int t = 0; t < NT; ++t) bw[t] = nw[t];
 #pragma unroll
       for (int m = 0; m < MT; ++m) bx[m] = nx[m];
     }
@@ -241,9 +249,9 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
   lds_loads_wait<0>();
   // a lane holds, of row row0 + (wr MT + m) 32 + r, columns 8 q + 4 g + 0..3 (q 0..3) of tile t
   if constexpr (!GATED) {
-    const int n_base = nblock * kTileCols + wc * 64;
+    const int n_base = nblock * kTileCols + wc * (32 * NT);
     if (n_base >= o.n_out) return;
-    // The results go through the wave's own part of LDS (everyone has read the last step), a row group at a time, to leave as whole lines of 128 bytes;
+    // The results go through the wave's own part of LDS (everyone has read the last step), a row group at a time, to leave as whole lines of 64 NT bytes;
     // a lane first exchanges halves with lane ^ 32, so that it has eight columns of its row.  Rows that do not begin at 16-byte addresses are
     // stored by elements.  (Stored from the registers, pieces of 16 bytes a row, 8,192 x 2,048 x 2,560 in one round of tiles took 49 us, so 39.)
     const bool wide = (o.n_out & 7) == 0 && ((uintptr_t)o.out & 15) == 0;
@@ -255,24 +263,25 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
       if (first >= row_end) break;                  // (the wave's)
       if (wide) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const f32x16& v = acc[t][m];
             const auto lo = __builtin_amdgcn_permlane32_swap(f32_to_bf16_pair(v[8 * h], v[8 * h + 1]), f32_to_bf16_pair(v[8 * h + 4], v[8 * h + 5]), false, false);
             const auto hi = __builtin_amdgcn_permlane32_swap(f32_to_bf16_pair(v[8 * h + 2], v[8 * h + 3]), f32_to_bf16_pair(v[8 * h + 6], v[8 * h + 7]), false, false);
-            *reinterpret_cast<uint4*>(mine + r * 128 + ((t * 4 + h * 2 + g) ^ (r & 7)) * 16) = make_uint4(lo[0], hi[0], lo[1], hi[1]);
+            *reinterpret_cast<uint4*>(mine + r * (64 * NT) + ((t * 4 + h * 2 + g) ^ (r & (4 * NT - 1))) * 16) = make_uint4(lo[0], hi[0], lo[1], hi[1]);
           }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int lrow = i * 8 + (lane >> 3), n = n_base + (lane & 7) * 8;
-          const uint4 v = *reinterpret_cast<const uint4*>(mine + lrow * 128 + ((lane & 7) ^ (lrow & 7)) * 16);
+        for (int i = 0; i < 2 * NT; ++i) {
+          constexpr int P = 4 * NT;                 // pieces of a row
+          const int lrow = i * (64 / P) + lane / P, n = n_base + lane % P * 8;
+          const uint4 v = *reinterpret_cast<const uint4*>(mine + lrow * (64 * NT) + (lane % P ^ (lrow & (P - 1))) * 16);
           if (first + lrow < row_end && n < o.n_out) *reinterpret_cast<uint4*>(o.out + (size_t)(first + lrow) * o.n_out + n) = v;
         }
       } else if (first + r < row_end) {
         bf16_t* dst = o.out + (size_t)(first + r) * o.n_out;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int n = n_base + t * 32 + (i / 4) * 8 + g * 4 + i % 4;
@@ -336,61 +345,80 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
 constexpr int kSideBySide = 4;
 constexpr int kDies = 8;
 
-template <bool GATED>
-__global__ __launch_bounds__(TW* kWave, 2) void fp8_tiles_kernel(F8Tiles p, F8Out o, GatedAct act) {
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[kTileLds];
-  __shared__ float s_top[GATED ? TWC : 1][64 * kHighest];
+template <int NT, bool GATED, bool PAIRED>
+__global__ __launch_bounds__(TW* kWave, PAIRED ? 4 : 2) void fp8_tiles_kernel(F8Tiles p, F8Out o, GatedAct act) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[Ring<PAIRED>::kLds];
+  __shared__ float s_top[GATED ? TWC : 1][64 * Ring<PAIRED>::kHighest];
   __shared__ int s_found[3];
   const int lane = threadIdx.x & (kWave - 1);
   const int slots = gridDim.x, die = blockIdx.x % kDies;
   const int slot = die * (slots / kDies) + min(die, slots % kDies) + blockIdx.x / kDies;
   const int c0 = slot / (kSideBySide * p.tiles) * kSideBySide, left = slot - c0 * p.tiles, wide = min(kSideBySide, p.nb - c0);
-  const int tile = left / wide, nblock = c0 + left % wide;
+  int tile = left / wide;
+  const int nblock = c0 + left % wide;
+  // the rows behind the list, whose tiles are bound by products, go evenly among the experts', which are bound by reading their weights
+  const int along = p.along > 0 ? (p.along + p.height - 1) / p.height : 0;
+  if (along) {
+    const int before = (int)((long long)tile * along / p.tiles);
+    if ((int)((long long)(tile + 1) * along / p.tiles) > before) tile = -1 - before;
+    else tile -= before;
+  }
   int e = 0, row0 = tile * p.height, row_end = min(p.rows, row0 + p.height);
   if (p.offsets) {
     // the groups' tiles are numbered through: as few of up to `height` rows as hold a group's, all of one height
-    if (threadIdx.x < kWave) {
-      int before = 0, found = -1, first_row = 0, last_row = 0;
-      for (int c = 0; c < p.groups + (p.along > 0) && found < 0; c += kWave) {
-        const int i = c + lane;
-        const int from = i < p.groups ? p.offsets[i] : p.rows, to = i < p.groups ? p.offsets[i + 1] : i == p.groups ? p.rows + p.along : p.rows;
-        const int mine = (to - from + p.height - 1) / p.height;
-        int upto = mine;
+    if (tile < 0) {
+      const int n = along, each = ((p.along + n - 1) / n + 63) & ~63;
+      e = p.groups;
+      row0 = p.rows + (-1 - tile) * each;
+      row_end = min(p.rows + p.along, row0 + each);
+    } else {
+      if (threadIdx.x < kWave) {
+        int before = 0, found = -1, first_row = 0, last_row = 0;
+        for (int c = 0; c < p.groups && found < 0; c += kWave) {
+          const int i = c + lane;
+          const int from = p.offsets[min(i, p.groups)], to = p.offsets[min(i + 1, p.groups)];
+          const int mine = (to - from + p.height - 1) / p.height;
+          int upto = mine;
 #pragma unroll
-        for (int k = 1; k < kWave; k <<= 1) {
-          const int up = __shfl_up(upto, k, kWave);
-          if (lane >= k) upto += up;
+          for (int k = 1; k < kWave; k <<= 1) {
+            const int up = __shfl_up(upto, k, kWave);
+            if (lane >= k) upto += up;
+          }
+          const int first = before + upto - mine;
+          const unsigned long long here = __builtin_amdgcn_ballot_w64(mine > 0 && tile >= first && tile < first + mine);
+          if (here) {
+            const int l = __ffsll((long long)here) - 1;
+            const int n = __shfl(mine, l, kWave), f = __shfl(from, l, kWave), t = __shfl(to, l, kWave);
+            const int each = ((t - f + n - 1) / n + 63) & ~63;
+            found = c + l;
+            first_row = f + (tile - __shfl(first, l, kWave)) * each;
+            last_row = min(t, first_row + each);
+          }
+          before += __shfl(upto, kWave - 1, kWave);
         }
-        const int first = before + upto - mine;
-        const unsigned long long here = __builtin_amdgcn_ballot_w64(mine > 0 && tile >= first && tile < first + mine);
-        if (here) {
-          const int l = __ffsll((long long)here) - 1;
-          const int n = __shfl(mine, l, kWave), f = __shfl(from, l, kWave), t = __shfl(to, l, kWave);
-          const int each = ((t - f + n - 1) / n + 63) & ~63;
-          found = c + l;
-          first_row = f + (tile - __shfl(first, l, kWave)) * each;
-          last_row = min(t, first_row + each);
+        if (threadIdx.x == 0) {
+          s_found[0] = found;
+          s_found[1] = first_row;
+          s_found[2] = last_row;
         }
-        before += __shfl(upto, kWave - 1, kWave);
       }
-      if (threadIdx.x == 0) {
-        s_found[0] = found;
-        s_found[1] = first_row;
-        s_found[2] = last_row;
-      }
+      __syncthreads();
+      e = __builtin_amdgcn_readfirstlane(s_found[0]);
+      row0 = __builtin_amdgcn_readfirstlane(s_found[1]);
+      row_end = __builtin_amdgcn_readfirstlane(s_found[2]);
+      if (e < 0) return;
     }
-    __syncthreads();
-    e = __builtin_amdgcn_readfirstlane(s_found[0]);
-    row0 = __builtin_amdgcn_readfirstlane(s_found[1]);
-    row_end = __builtin_amdgcn_readfirstlane(s_found[2]);
-    if (e < 0) return;
   }
   const int rows = row_end - row0;
   if (rows <= 0) return;
-  if (rows <= 64) f8_tile<1, GATED>(p, o, act, e, row0, row_end, nblock, smem, s_top);
-  else if (rows <= 128) f8_tile<2, GATED>(p, o, act, e, row0, row_end, nblock, smem, s_top);
-  else if (rows <= 192) f8_tile<3, GATED>(p, o, act, e, row0, row_end, nblock, smem, s_top);
-  else f8_tile<4, GATED>(p, o, act, e, row0, row_end, nblock, smem, s_top);
+#define F8_TILE(MTV) f8_tile<MTV, NT, GATED, PAIRED>(p, o, act, e, row0, row_end, nblock, smem, s_top)
+  if (rows <= 64) F8_TILE(1);
+  else if (PAIRED || rows <= 128) F8_TILE(2);
+  else if constexpr (!PAIRED) {
+    if (rows <= 192) F8_TILE(3);
+    else F8_TILE(4);
+  }
+#undef F8_TILE
 }
 
 bool tiles_ok(const F8Tiles& p, int x_rows) {
@@ -399,16 +427,19 @@ bool tiles_ok(const F8Tiles& p, int x_rows) {
          (!p.a_rows || (long long)x_rows * p.U * kF8Block <= 0xffffffffLL) && (long long)p.U * kF8TileBytes <= 0x7fffffffLL;
 }
 
-template <bool GATED> int launch_tiles(F8Tiles p, const F8Out& o, GatedAct act, hipStream_t stream) {
+template <bool GATED> int launch_tiles(F8Tiles p, const F8Out& o, GatedAct act, int nt, hipStream_t stream) {
   const int height = p.height;
-  if (height < 64 || height > 64 * kHighest || height % 64) return SHARPI_ERR_ARG;
+  if (height < 64 || height > 64 * Ring<false>::kHighest || height % 64) return SHARPI_ERR_ARG;
   const long long tiles = p.offsets ? (long long)p.rows / height + (p.rows < p.groups ? p.rows : p.groups) + (p.along + height - 1) / height
                                     : (p.rows + height - 1) / height;
-  p.nb = ceil_div(o.n_out, GATED ? kTileCols / 2 : kTileCols);
+  if ((nt != 1 && nt != 2) || (nt == 1 && (GATED || height <= 64 * Ring<true>::kHighest))) return SHARPI_ERR_ARG;
+  p.nb = ceil_div(o.n_out, GATED ? columns_of(nt) / 2 : columns_of(nt));
   p.tiles = (int)tiles;
   if (tiles * p.nb > 0x7fffffffLL) return SHARPI_ERR_ARG;
   const dim3 grid((unsigned)(tiles * p.nb)), block(TW * kWave);
-  fp8_tiles_kernel<GATED><<<grid, block, 0, stream>>>(p, o, act);
+  if (height <= 64 * Ring<true>::kHighest) fp8_tiles_kernel<2, GATED, true><<<grid, block, 0, stream>>>(p, o, act);
+  else if (nt == 2) fp8_tiles_kernel<2, GATED, false><<<grid, block, 0, stream>>>(p, o, act);
+  else if constexpr (!GATED) fp8_tiles_kernel<1, GATED, false><<<grid, block, 0, stream>>>(p, o, act);
   SHARPI_CHECK_LAUNCH();
   return SHARPI_OK;
 }
@@ -416,14 +447,14 @@ template <bool GATED> int launch_tiles(F8Tiles p, const F8Out& o, GatedAct act, 
 }  // namespace
 
 // out [rows, N] bfloat16.  x: codes [x_rows, 128 U] and scales; w_rows: stored rows of one matrix; a_rows, offsets: of a sorted row list, or null; along: rows
-// behind the list's `rows`, which matrix `groups` takes (row i reads row i - rows of x if there is a_rows); height: rows of a tile at most (64, 128, 192, 256).
+// behind the list's `rows`, which matrix `groups` takes (row i reads row i - rows of x if there is a_rows); height: rows of a tile at most (64, 128, 192, 256); nt: its columns, 128 nt (1 with heights from 192 on).
 SHARPI_EXPORT int sharpi_fp8_tiles(const void* x, const void* x_scales, int x_rows, const void* w_codes, const void* w_scales, int w_rows, void* out,
-                                   int rows, int N, int K, const int* a_rows, const int* offsets, int groups, int along, int height, hipStream_t stream) {
+                                   int rows, int N, int K, const int* a_rows, const int* offsets, int groups, int along, int height, int nt, hipStream_t stream) {
   if (rows <= 0) return SHARPI_OK;
   if (N <= 0 || K <= 0 || w_rows != f8_padded_rows(N)) return SHARPI_ERR_ARG;
   const F8Tiles p{(const uint8_t*)x, (const uint8_t*)x_scales, (const uint8_t*)w_codes, (const uint8_t*)w_scales, f8_blocks(K), w_rows, a_rows, offsets, rows, groups, (uint32_t)((long long)x_rows * f8_blocks(K) * kF8Block), along, height, 0, 0};
   if (!tiles_ok(p, x_rows)) return SHARPI_ERR_ARG;
-  return launch_tiles<false>(p, F8Out{(bf16_t*)out, nullptr, nullptr, nullptr, N}, GatedAct{}, stream);
+  return launch_tiles<false>(p, F8Out{(bf16_t*)out, nullptr, nullptr, nullptr, N}, GatedAct{}, nt, stream);
 }
 
 // codes [rows, 128 f8_blocks(I)] and scales [rows, f8_scale_stride(I)] of act(s g) (s u); w_rows: twice I up to a multiple of 32; score [rows] or null.
@@ -435,5 +466,5 @@ SHARPI_EXPORT int sharpi_fp8_tiles_gated(const void* x, const void* x_scales, in
   if (I <= 0 || K <= 0 || w_rows != 2 * f8_padded_rows(I) || !act_known(ga) || ((uintptr_t)codes & 15)) return SHARPI_ERR_ARG;
   const F8Tiles p{(const uint8_t*)x, (const uint8_t*)x_scales, (const uint8_t*)w_codes, (const uint8_t*)w_scales, f8_blocks(K), w_rows, a_rows, offsets, rows, groups, (uint32_t)((long long)x_rows * f8_blocks(K) * kF8Block), along, height, 0, 0};
   if (!tiles_ok(p, x_rows)) return SHARPI_ERR_ARG;
-  return launch_tiles<true>(p, F8Out{nullptr, (uint8_t*)codes, (uint8_t*)scales, score, I}, ga, stream);
+  return launch_tiles<true>(p, F8Out{nullptr, (uint8_t*)codes, (uint8_t*)scales, score, I}, ga, 2, stream);
 }

@@ -10,11 +10,13 @@ are some 2^-13 of the largest.
 from __future__ import annotations
 
 import contextlib
-from typing import Optional, Union
+import functools
+import math
+from typing import Optional, Tuple, Union
 
 import torch
 
-from . import ACT_SILU, _code, _dev, _i32, _known_act_pair, _need, _ptr, _run, _stream, compute_units
+from . import ACT_SILU, _code, _dev, _i32, _known_act_pair, _need, _ptr, _run, compute_units
 
 FP8_BLOCK = 128                # values that share a scale
 FP8_TILE = 32                  # weight rows of a stored tile
@@ -44,7 +46,39 @@ def _powers(s: torch.Tensor) -> torch.Tensor:
 
 def _device_of(t: torch.Tensor):
     """The launches of a call go to its tensors' device."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _NOTHING if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+_NOTHING = contextlib.nullcontext()
+# (the handle of a device's current stream without a Stream object around it: 0.1 us for 2.8)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream_of(t: torch.Tensor) -> int:
+    """The current stream of the tensor's device."""
+    return _raw_stream(t.device.index) if _raw_stream is not None else torch.cuda.current_stream(t.device).cuda_stream
+
+
+class _Scratch:
+    """Buffers of one call in one allocation, by address: what a call's launches hand to one another."""
+
+    __slots__ = ("memory", "base", "size")
+
+    def __init__(self):
+        self.memory, self.base, self.size = None, 0, 0
+
+    def add(self, nbytes: int) -> int:
+        """Offset of a further buffer of so many bytes, on a border of 256."""
+        at = self.size
+        self.size = at + -(-nbytes // 256) * 256
+        return at
+
+    def make(self, device) -> None:
+        self.memory = torch.empty(max(self.size, 1), dtype=torch.uint8, device=device)
+        self.base = self.memory.data_ptr()
+
+    def __getitem__(self, at: int) -> int:
+        return self.base + at
 
 
 def _same_device(*ts) -> None:
@@ -165,8 +199,11 @@ def quantize_weight(w: torch.Tensor, gated: bool = False) -> Fp8Weight:
 
 
 def _new_rows(M: int, k: int, device) -> Fp8Rows:
-    return Fp8Rows(torch.empty(M, _blocks(k) * FP8_BLOCK, dtype=torch.float8_e4m3fn, device=device),
-                   torch.empty(M, _scale_stride(k), dtype=torch.uint8, device=device), k)
+    q = object.__new__(Fp8Rows)
+    q.codes = torch.empty((M, _blocks(k) * FP8_BLOCK), dtype=torch.float8_e4m3fn, device=device)
+    q.scales = torch.empty((M, _scale_stride(k)), dtype=torch.uint8, device=device)
+    q.shape = (M, k)
+    return q
 
 
 def quantize_rows(x: torch.Tensor, act=None) -> Fp8Rows:
@@ -180,24 +217,37 @@ def quantize_rows(x: torch.Tensor, act=None) -> Fp8Rows:
     M, K = x.shape[0], x.shape[1] // (2 if code else 1)
     out = _new_rows(M, K, x.device)
     with _device_of(x):
-        _run("sharpi_fp8_rows", _ptr(x), dt, _ptr(out.codes), _ptr(out.scales), M, K, code, limit, _stream())
+        _run("sharpi_fp8_rows", x.data_ptr(), dt, out.codes.data_ptr(), out.scales.data_ptr(), M, K, code, limit, _stream_of(x))
     return out
 
 
-def _rows_of(x) -> Fp8Rows:
-    return x if isinstance(x, Fp8Rows) else quantize_rows(x)
+def _staged(x) -> bool:
+    """Whether the weight-streaming kernels quantise these rows where they are read: up to 16 rows of bfloat16 that fit in LDS."""
+    return (isinstance(x, torch.Tensor) and x.dtype == torch.bfloat16 and x.shape[0] <= 16 and x.shape[1] % 8 == 0 and x.data_ptr() % 16 == 0
+            and x.shape[0] * _blocks(x.shape[1]) * (FP8_BLOCK + 1) + 16 <= FP8_STAGED_BYTES)
 
 
-def _few_rows_of(x):
-    """(tensor, scales, kind) of the rows as the weight-streaming kernels take them: up to 16 rows of bfloat16 are quantised where they are read, if they
-    fit in LDS."""
-    if isinstance(x, Fp8Rows):
-        return x.codes, x.scales, _X_CODES
-    if (x.dtype == torch.bfloat16 and x.shape[0] <= 16 and x.shape[1] % 8 == 0 and x.data_ptr() % 16 == 0
-            and x.shape[0] * _blocks(x.shape[1]) * (FP8_BLOCK + 1) + 16 <= FP8_STAGED_BYTES):
-        return x, None, _code(x.dtype)
-    q = quantize_rows(x)
-    return q.codes, q.scales, _X_CODES
+class _Operand:
+    """The rows of a product as its kernel takes them: (address, scales' address, kind); quantised into the call's scratch memory if they are
+    not codes yet and ``staged`` does not hold."""
+
+    __slots__ = ("x", "staged", "codes_at", "scales_at")
+
+    def __init__(self, x, scratch: _Scratch, staged: bool):
+        self.x, self.staged = x, staged
+        if isinstance(x, torch.Tensor) and not staged:
+            M, k = x.shape
+            self.codes_at, self.scales_at = scratch.add(M * _blocks(k) * FP8_BLOCK), scratch.add(M * _scale_stride(k))
+
+    def ready(self, scratch: _Scratch, stream: int) -> Tuple[int, Optional[int], int]:
+        x = self.x
+        if not isinstance(x, torch.Tensor):
+            return x.codes.data_ptr(), x.scales.data_ptr(), _X_CODES
+        if self.staged:
+            return x.data_ptr(), None, _code(x.dtype)
+        codes, scales = scratch[self.codes_at], scratch[self.scales_at]
+        _run("sharpi_fp8_rows", x.data_ptr(), _code(x.dtype), codes, scales, x.shape[0], x.shape[1], 0, 0.0, stream)
+        return codes, scales, _X_CODES
 
 
 def _rows_checked(x, k: int, who: str) -> None:
@@ -210,23 +260,35 @@ def _rows_checked(x, k: int, who: str) -> None:
 
 
 def linear_fp8(x: Union[torch.Tensor, Fp8Rows], w: Fp8Weight) -> torch.Tensor:
-    """x [M, K] W^T in 8 bits: bfloat16 [M, N]."""
+    """x [M, K] W^T in 8 bits: bfloat16 [M, N].  A few rows go by streaming the weights, more in tiles (``few_rows_fp8``, ``tile_fp8``)."""
     _need(isinstance(w, Fp8Weight) and w.dim() == 2 and not w.gated, "linear_fp8: w must be an Fp8Weight [N, K], not gated")
     N, K = w.shape
     _rows_checked(x, K, "linear_fp8")
-    _same_device(w.codes, x if isinstance(x, torch.Tensor) else x.codes)
     M = x.shape[0]
-    out = torch.empty(M, N, dtype=torch.bfloat16, device=w.device)
+    _same_device(w.codes, x if isinstance(x, torch.Tensor) else x.codes)
+    out = torch.empty((M, N), dtype=torch.bfloat16, device=w.codes.device)
+    if M == 0:
+        return out
+    few = few_rows_fp8(M, N)
+    scratch = _Scratch()
+    rows = _Operand(x, scratch, few and _staged(x))
+    if scratch.size:
+        scratch.make(out.device)
     with _device_of(out):
-        if M <= FP8_FEW_ROWS:
-            rows, scales, kind = _few_rows_of(x)
-            _run("sharpi_fp8_few", _ptr(rows), _ptr(scales), kind, _ptr(w.codes), _ptr(w.scales), w.stored_rows, _ptr(out), M, N, K,
-                 _few_tiles(N), _stream())
+        stream = _stream_of(out)
+        a, scales, kind = rows.ready(scratch, stream)
+        if few:
+            _run("sharpi_fp8_few", a, scales, kind, w.codes.data_ptr(), w.scales.data_ptr(), w.stored_rows, out.data_ptr(), M, N, K,
+                 _few_tiles(N), stream)
         else:
-            q = _rows_of(x)
-            _run("sharpi_fp8_tiles", _ptr(q.codes), _ptr(q.scales), M, _ptr(w.codes), _ptr(w.scales), w.stored_rows, _ptr(out), M, N, K,
-                 None, None, 1, 0, _height(M, 1), _stream())
+            _run("sharpi_fp8_tiles", a, scales, M, w.codes.data_ptr(), w.scales.data_ptr(), w.stored_rows, out.data_ptr(), M, N, K,
+                 None, None, 1, 0, *tile_fp8(M, N, K, False, compute_units()), stream)
     return out
+
+
+def few_rows_fp8(M: int, N: int) -> bool:
+    """Whether a product of M rows goes by streaming the weights."""
+    return M <= FP8_FEW_ROWS
 
 
 def _few_tiles(N: int) -> int:
@@ -234,10 +296,36 @@ def _few_tiles(N: int) -> int:
     return 2 if N >= 16384 else 1
 
 
-def _height(rows: int, groups: int) -> int:
-    """Rows of a tile."""
-    each = rows / groups
-    return 64 if each <= 64 else 128 if each <= 128 else 256
+# us that a step of 64 of k takes in a tile, where it runs alone on the chip and where all compute units do, by (rows / 64, columns / 128); tiles of up to 128
+# rows in pairs of blocks a unit
+TILE_STEP_US = {(1, 1): (0.24, 0.36), (2, 1): (0.28, 0.39), (3, 1): (0.39, 0.41), (4, 1): (0.42, 0.53), (3, 2): (0.50, 0.60), (4, 2): (0.59, 0.75)}
+PAIRED_STEP_US = {1: (0.38, 0.62), 2: (0.42, 0.86)}
+TILE_END_US = 5.0
+
+
+@functools.lru_cache(maxsize=1024)
+def tile_fp8(M: int, N: int, K: int, gated: bool, units: int) -> Tuple[int, int]:
+    """(rows, columns / 128) of the tiles of a product of many rows (gated: 256 columns): those whose rounds of the chip take the least time."""
+    steps = 2 * _blocks(K)
+
+    def expected(height: int, nt: int) -> float:
+        blocks = -(-M // height) * -(-N // (128 if gated else 128 * nt))
+        tall = -(-min(M, height) // 64)
+        low, full = PAIRED_STEP_US[tall] if height <= 128 else TILE_STEP_US[(tall, nt)] if (tall, nt) in TILE_STEP_US else TILE_STEP_US[(3, nt)]
+        at_once = 2 * units if height <= 128 else units
+        rounds, rest = divmod(blocks, at_once)
+        us = rounds * (full * steps + TILE_END_US)
+        if rest:
+            fill = max(0.0, (rest - units) / units) if height <= 128 else rest / units
+            us += (low + (full - low) * fill) * steps + TILE_END_US
+        return us
+    choices = [(64, 2), (128, 2), (192, 2), (256, 2)] + ([] if gated else [(192, 1), (256, 1)])
+    return min(choices, key=lambda c: expected(*c))
+
+
+def grouped_tile_fp8(rows: int, groups: int) -> int:
+    """Rows of the tiles of a layer's products at most."""
+    return 128 if rows <= 96 * groups else 256
 
 
 def _layer_checked(x, w_gate_up: Fp8Weight, w_down: Fp8Weight, dims: int, who: str):
@@ -252,30 +340,40 @@ def _layer_checked(x, w_gate_up: Fp8Weight, w_down: Fp8Weight, dims: int, who: s
 
 def _few_layer(x, ids, wts, w1: Fp8Weight, w2: Fp8Weight, code: int, limit: float, on_input: bool, shared: bool, E: int) -> torch.Tensor:
     T, K, inner, N = x.shape[0], w1.shape[-1], w1.shape[-2] // 2, w2.shape[-2]
-    k = 1 if ids is None else ids.shape[1]
-    rows = T * k + (T if shared else 0)
-    stride = -(-inner // 8) * 8
-    R = 2
-    tiles = -(-N // (16 * R))
-    met = (min(E, T * k) + (1 if shared else 0)) if ids is not None else 1
-    S = max(1, min(2 * compute_units() // tiles, met * _blocks(inner) // 8))
+    k, also = 1 if ids is None else ids.shape[1], 1 if shared else 0
+    rows, stride = T * k + also * T, -(-inner // 8) * 8
+    met = min(E, T * k) + also if ids is not None else 1
+    tiles = -(-N // (16 * SUM_TILES))
+    shares = sum_shares(tiles, met * _blocks(inner), compute_units())
     row_blocks = 1 if T <= 16 else 2 if T <= 32 else 4
-    h = torch.empty(rows, stride, dtype=torch.bfloat16, device=w1.device)
-    out = torch.empty(T, N, dtype=torch.bfloat16, device=w1.device)
-    counters = torch.empty(tiles, dtype=torch.int32, device=w1.device)
-    part = torch.empty(S * tiles * R * row_blocks * 256 if S > 1 else 1, dtype=torch.float32, device=w1.device)
-    a, scales, kind = _few_rows_of(x)
-    w_in, w_out = (wts, None) if on_input else (None, wts)
-    _run("sharpi_fp8_few_gated", _ptr(a), _ptr(scales), kind, _ptr(w1.codes), _ptr(w1.scales), w1.stored_rows, _ptr(h), stride, _ptr(ids), _ptr(w_in),
-         T, k, E, 1 if shared else 0, inner, K, code, limit, 2, _ptr(counters), tiles, _stream())
-    if T <= 16:
-        a, scales, kind = h, None, _code(h.dtype)
-    else:
-        q = quantize_rows(h)
-        a, scales, kind = q.codes, q.scales, _X_CODES
-    _run("sharpi_fp8_few_sum", _ptr(a), _ptr(scales), kind, _ptr(w2.codes), _ptr(w2.scales), w2.stored_rows, _ptr(out), _ptr(ids), _ptr(w_out), T, k, E,
-         1 if shared else 0, N, stride, R, S, _ptr(part), _ptr(counters), _stream())
+    scratch = _Scratch()
+    h, counters = scratch.add(rows * stride * 2), scratch.add(tiles * 4)
+    part = scratch.add(shares * tiles * SUM_TILES * row_blocks * 1024 if shares > 1 else 0)
+    operand = _Operand(x, scratch, _staged(x))
+    if T > 16:
+        codes, scales_at = scratch.add(rows * _blocks(stride) * FP8_BLOCK), scratch.add(rows * _scale_stride(stride))
+    scratch.make(w1.codes.device)
+    out = torch.empty((T, N), dtype=torch.bfloat16, device=w1.codes.device)
+    stream, ids_at = _stream_of(out), _ptr(ids)
+    a, scales, kind = operand.ready(scratch, stream)
+    w_in, w_out = (_ptr(wts), None) if on_input else (None, _ptr(wts))
+    _run("sharpi_fp8_few_gated", a, scales, kind, w1.codes.data_ptr(), w1.scales.data_ptr(), w1.stored_rows, scratch[h], stride, ids_at, w_in,
+         T, k, E, also, inner, K, code, limit, 2, scratch[counters], tiles, stream)
+    a, scales, kind = scratch[h], None, _code(torch.bfloat16)
+    if T > 16:
+        a, scales, kind = scratch[codes], scratch[scales_at], _X_CODES
+        _run("sharpi_fp8_rows", scratch[h], _code(torch.bfloat16), a, scales, rows, stride, 0, 0.0, stream)
+    _run("sharpi_fp8_few_sum", a, scales, kind, w2.codes.data_ptr(), w2.scales.data_ptr(), w2.stored_rows, out.data_ptr(), ids_at, w_out, T, k, E,
+         also, N, stride, SUM_TILES, shares, scratch[part], scratch[counters], stream)
     return out
+
+
+SUM_TILES = 2        # half tiles of 16 columns a block of the sum takes
+
+
+def sum_shares(tiles: int, blocks: int, units: int) -> int:
+    """Shares of the blocks of k that a layer's second product is dealt to for each column tile: about two blocks a compute unit, of eight or more."""
+    return max(1, min(2 * units // tiles, blocks // 8))
 
 
 def feed_forward_fp8(x: Union[torch.Tensor, Fp8Rows], w_gate_up: Fp8Weight, w_down: Fp8Weight, act=ACT_SILU) -> torch.Tensor:
@@ -288,10 +386,18 @@ def feed_forward_fp8(x: Union[torch.Tensor, Fp8Rows], w_gate_up: Fp8Weight, w_do
             return torch.empty(0, N, dtype=torch.bfloat16, device=w_down.device)
         if M <= FP8_FEW_ROWS:
             return _few_layer(x, None, None, w_gate_up, w_down, code, limit, False, False, 1)
-        q, h = _rows_of(x), _new_rows(M, inner, w_down.device)
-        _run("sharpi_fp8_tiles_gated", _ptr(q.codes), _ptr(q.scales), M, _ptr(w_gate_up.codes), _ptr(w_gate_up.scales), w_gate_up.stored_rows, _ptr(h.codes),
-             _ptr(h.scales), M, inner, K, None, None, 1, 0, None, code, limit, _height(M, 1), _stream())
-        return linear_fp8(h, w_down)
+        scratch = _Scratch()
+        operand = _Operand(x, scratch, False)
+        codes, scales = scratch.add(M * _blocks(inner) * FP8_BLOCK), scratch.add(M * _scale_stride(inner))
+        scratch.make(w_down.codes.device)
+        out = torch.empty((M, N), dtype=torch.bfloat16, device=w_down.codes.device)
+        stream = _stream_of(out)
+        a, a_scales, _ = operand.ready(scratch, stream)
+        _run("sharpi_fp8_tiles_gated", a, a_scales, M, w_gate_up.codes.data_ptr(), w_gate_up.scales.data_ptr(), w_gate_up.stored_rows, scratch[codes],
+             scratch[scales], M, inner, K, None, None, 1, 0, None, code, limit, tile_fp8(M, inner, K, True, compute_units())[0], stream)
+        _run("sharpi_fp8_tiles", scratch[codes], scratch[scales], M, w_down.codes.data_ptr(), w_down.scales.data_ptr(), w_down.stored_rows, out.data_ptr(),
+             M, N, inner, None, None, 1, 0, *tile_fp8(M, N, inner, False, compute_units()), stream)
+        return out
 
 
 def experts_fp8(x: Union[torch.Tensor, Fp8Rows], ids: torch.Tensor, wts: torch.Tensor, w_gate_up: Fp8Weight, w_down: Fp8Weight, act=ACT_SILU,
@@ -317,25 +423,29 @@ def experts_fp8(x: Union[torch.Tensor, Fp8Rows], ids: torch.Tensor, wts: torch.T
             return torch.empty(0, N, dtype=torch.bfloat16, device=w_down.device)
         if T <= FP8_FEW_ROWS and T * k <= FP8_FEW_PAIRS:
             return _few_layer(x, ids, wts, w_gate_up, w_down, code, limit, score_on_input, shared, E)
-        return _many_layer(_rows_of(x), ids, wts, w_gate_up, w_down, code, limit, score_on_input, shared, E, inner, N)
+        return _many_layer(x, ids, wts, w_gate_up, w_down, code, limit, score_on_input, shared, E, inner, N)
 
 
-def _many_layer(q: Fp8Rows, ids, wts, w1: Fp8Weight, w2: Fp8Weight, code: int, limit: float, on_input: bool, shared: bool, E: int, inner: int, N: int) -> torch.Tensor:
+def _many_layer(x, ids, wts, w1: Fp8Weight, w2: Fp8Weight, code: int, limit: float, on_input: bool, shared: bool, E: int, inner: int, N: int) -> torch.Tensor:
     T, k = ids.shape
-    n, along, dev = T * k, T if shared else 0, w1.device
+    n, along, dev = T * k, T if shared else 0, w1.codes.device
     # the picks sorted by expert (no plan: that is the bfloat16 product's); the always-on matrix takes the tokens behind them, in their order
-    ints = torch.empty(E + 1 + 2 * n, dtype=torch.int32, device=dev)
-    offsets, tokens, inv_pos = ints[:E + 1], ints[E + 1:E + 1 + n], ints[E + 1 + n:]
-    scores = torch.empty(n, dtype=torch.float32, device=dev)
-    _run("sharpi_moe_permute", _ptr(ids), _ptr(wts), _ptr(offsets), _ptr(tokens), _ptr(scores), _ptr(inv_pos), None, 0, T, k, E, 0, 1, _stream())
-    height = _height(n, E)
-    h = _new_rows(n + along, inner, dev)
-    _run("sharpi_fp8_tiles_gated", _ptr(q.codes), _ptr(q.scales), T, _ptr(w1.codes), _ptr(w1.scales), w1.stored_rows, _ptr(h.codes), _ptr(h.scales),
-         n, inner, w1.shape[-1], _ptr(tokens), _ptr(offsets), E, along, _ptr(scores) if on_input else None, code, limit, height, _stream())
-    y = torch.empty(n + along, N, dtype=torch.bfloat16, device=dev)
-    _run("sharpi_fp8_tiles", _ptr(h.codes), _ptr(h.scales), n + along, _ptr(w2.codes), _ptr(w2.scales), w2.stored_rows, _ptr(y), n, N, inner,
-         None, _ptr(offsets), E, along, height, _stream())
-    out = torch.empty(T, N, dtype=torch.bfloat16, device=dev)
-    _run("sharpi_fp8_combine", _ptr(y), _ptr(inv_pos), _ptr(ids), _ptr(y[n:]) if shared else None, None if on_input else _ptr(wts), _ptr(out),
-         T, N, k, E, _stream())
+    scratch = _Scratch()
+    operand = _Operand(x, scratch, False)
+    offsets, tokens, inv_pos, scores = scratch.add((E + 1) * 4), scratch.add(n * 4), scratch.add(n * 4), scratch.add(n * 4)
+    codes, scales = scratch.add((n + along) * _blocks(inner) * FP8_BLOCK), scratch.add((n + along) * _scale_stride(inner))
+    y = scratch.add((n + along) * N * 2)
+    shared_y = y + n * N * 2
+    scratch.make(dev)
+    out = torch.empty((T, N), dtype=torch.bfloat16, device=dev)
+    stream, height = _stream_of(out), grouped_tile_fp8(n, E)
+    a, a_scales, _ = operand.ready(scratch, stream)
+    _run("sharpi_moe_permute", ids.data_ptr(), wts.data_ptr(), scratch[offsets], scratch[tokens], scratch[scores], scratch[inv_pos], None, 0,
+         T, k, E, 0, 1, stream)
+    _run("sharpi_fp8_tiles_gated", a, a_scales, T, w1.codes.data_ptr(), w1.scales.data_ptr(), w1.stored_rows, scratch[codes], scratch[scales],
+         n, inner, w1.shape[-1], scratch[tokens], scratch[offsets], E, along, scratch[scores] if on_input else None, code, limit, height, stream)
+    _run("sharpi_fp8_tiles", scratch[codes], scratch[scales], n + along, w2.codes.data_ptr(), w2.scales.data_ptr(), w2.stored_rows, scratch[y], n, N, inner,
+         None, scratch[offsets], E, along, height, 2, stream)
+    _run("sharpi_fp8_combine", scratch[y], scratch[inv_pos], ids.data_ptr(), scratch[shared_y] if shared else None, None if on_input else wts.data_ptr(),
+         out.data_ptr(), T, N, k, E, stream)
     return out
