@@ -86,11 +86,11 @@ SHARPI_EXPORT int sharpi_fp8_rows(const void* x, int dtype, void* codes, void* s
   return SHARPI_OK;
 }
 
-// out[t] = sum_j w[t, j] y[inv_pos[t, j]] (+ shared[t]) of bfloat16 rows, the sum in float; picks of n_experts and above have no row and add nothing.
+// out[t] = sum_j w[t, j] y[inv_pos[t, j]] (+ shared[t]) of float rows, rounded to bfloat16 once; picks of n_experts and above have no row and add nothing.
 // Bound: a pass over the rows.
 template <bool WIDE>
-__global__ __launch_bounds__(256) void fp8_combine_kernel(const bf16_t* __restrict__ y, const int* __restrict__ inv_pos, const int* __restrict__ ids,
-                                                          const bf16_t* __restrict__ shared, const float* __restrict__ w, bf16_t* __restrict__ out,
+__global__ __launch_bounds__(256) void fp8_combine_kernel(const float* __restrict__ y, const int* __restrict__ inv_pos, const int* __restrict__ ids,
+                                                          const float* __restrict__ shared, const float* __restrict__ w, bf16_t* __restrict__ out,
                                                           int columns, int k, int n_experts) {
   constexpr int V = WIDE ? 8 : 1;
   const size_t t = blockIdx.x;
@@ -99,10 +99,10 @@ __global__ __launch_bounds__(256) void fp8_combine_kernel(const bf16_t* __restri
   float acc[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
-  auto add = [&](const bf16_t* row, float weight) {
+  auto add = [&](const float* row, float weight) {
     float v[V];
     if constexpr (WIDE) load8(row + c, v);
-    else v[0] = to_f32(row[c]);
+    else v[0] = row[c];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = fmaf(weight, v[i], acc[i]);
   };
@@ -115,14 +115,14 @@ __global__ __launch_bounds__(256) void fp8_combine_kernel(const bf16_t* __restri
   else out[t * columns + c] = f32_to_bf16(acc[0]);
 }
 
-SHARPI_EXPORT int sharpi_fp8_combine(const void* y, const int* inv_pos, const int* ids, const void* shared, const float* w, void* out, int n_tokens,
+SHARPI_EXPORT int sharpi_fp8_combine(const float* y, const int* inv_pos, const int* ids, const float* shared, const float* w, void* out, int n_tokens,
                                      int columns, int k, int n_experts, hipStream_t stream) {
   if (n_tokens <= 0) return SHARPI_OK;
   if (columns <= 0 || k <= 0) return SHARPI_ERR_ARG;
   const bool wide = columns % 8 == 0 && (((uintptr_t)y | (uintptr_t)out | (uintptr_t)shared) & 15) == 0;
   const dim3 grid((unsigned)n_tokens, (unsigned)ceil_div(columns, wide ? 2048 : 256)), block(256);
-  if (wide) fp8_combine_kernel<true><<<grid, block, 0, stream>>>((const bf16_t*)y, inv_pos, ids, (const bf16_t*)shared, w, (bf16_t*)out, columns, k, n_experts);
-  else fp8_combine_kernel<false><<<grid, block, 0, stream>>>((const bf16_t*)y, inv_pos, ids, (const bf16_t*)shared, w, (bf16_t*)out, columns, k, n_experts);
+  if (wide) fp8_combine_kernel<true><<<grid, block, 0, stream>>>(y, inv_pos, ids, shared, w, (bf16_t*)out, columns, k, n_experts);
+  else fp8_combine_kernel<false><<<grid, block, 0, stream>>>(y, inv_pos, ids, shared, w, (bf16_t*)out, columns, k, n_experts);
   SHARPI_CHECK_LAUNCH();
   return SHARPI_OK;
 }

@@ -1,6 +1,6 @@
 // Products of many rows with weights in 8-bit floating point (fp8.h holds the format), in tiles on the scaled matrix instruction: one matrix, or
 // the experts of a routing's sorted row list.  Two forms:
-//   plain   out[row, :] = rows[row] W_e^T, bfloat16
+//   plain   out[row, :] = rows[row] W_e^T, bfloat16, or float where experts' outputs are still to be added up
 //   gated   act(s g) (s u) with (g | u) the product, rounded to bfloat16 and quantised again: codes and scale bytes of the rows that the
 //           second half of a feed-forward reads.  A block's 128 output columns are one block of the format, so the epilogue has what
 //           it needs, and neither (g | u) nor the unquantised rows go to memory.
@@ -32,9 +32,9 @@ struct F8Tiles {
   int tiles, nb;             // row tiles in all at most; column blocks
 };
 
-// plain: out [rows, n_out].  gated: codes [rows, 128 f8_blocks(n_out)], scales [rows, f8_scale_stride(n_out)], score [rows] or null.
+// plain: out [rows, n_out], bfloat16 or float.  gated: codes [rows, 128 f8_blocks(n_out)], scales [rows, f8_scale_stride(n_out)], score [rows] or null.
 struct F8Out {
-  bf16_t* out;
+  void* out;
   uint8_t* codes;
   uint8_t* scales;
   const float* score;
@@ -61,7 +61,7 @@ template <bool PAIRED> struct Ring {
 };
 
 // One tile: rows row0 .. row_end (up to 64 MT of them) of matrix e against column block nblock.  MT: groups of 32 rows a wave; NT: weight tiles of a wave.
-template <int MT, int NT, bool GATED, bool PAIRED>
+template <int MT, int NT, bool GATED, bool PAIRED, typename TO>
 __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedAct act, int e, int row0, int row_end, int nblock, unsigned char* smem,
                                         float (*s_top)[64 * Ring<PAIRED>::kHighest]) {
   using RG = Ring<PAIRED>;
@@ -254,38 +254,47 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
     // The results go through the wave's own part of LDS (everyone has read the last step), a row group at a time, to leave as whole lines of 64 NT bytes;
     // a lane first exchanges halves with lane ^ 32, so that it has eight columns of its row.  Rows that do not begin at 16-byte addresses are
     // stored by elements.  (Stored from the registers, pieces of 16 bytes a row, 8,192 x 2,048 x 2,560 in one round of tiles took 49 us, so 39.)
-    const bool wide = (o.n_out & 7) == 0 && ((uintptr_t)o.out & 15) == 0;
+    constexpr int V = 16 / sizeof(TO), P = 32 * NT / V;      // columns of a 16-byte piece, pieces of a row
+    TO* out = (TO*)o.out;
+    const bool wide = o.n_out % V == 0 && ((uintptr_t)out & 15) == 0;
     __syncthreads();
-    unsigned char* mine = smem + wid * 4096;
+    unsigned char* mine = smem + wid * (32 * P * 16);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int first = row0 + (wr * MT + m) * 32;
       if (first >= row_end) break;                  // (the wave's)
       if (wide) {
+        auto keep = [&](int piece, const uint4& v) { *reinterpret_cast<uint4*>(mine + r * (P * 16) + (piece ^ (r & (P < 8 ? P - 1 : 7))) * 16) = v; };
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t) {
+          const f32x16& v = acc[t][m];
+          if constexpr (sizeof(TO) == 4) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const f32x16& v = acc[t][m];
-            const auto lo = __builtin_amdgcn_permlane32_swap(f32_to_bf16_pair(v[8 * h], v[8 * h + 1]), f32_to_bf16_pair(v[8 * h + 4], v[8 * h + 5]), false, false);
-            const auto hi = __builtin_amdgcn_permlane32_swap(f32_to_bf16_pair(v[8 * h + 2], v[8 * h + 3]), f32_to_bf16_pair(v[8 * h + 6], v[8 * h + 7]), false, false);
-            *reinterpret_cast<uint4*>(mine + r * (64 * NT) + ((t * 4 + h * 2 + g) ^ (r & (4 * NT - 1))) * 16) = make_uint4(lo[0], hi[0], lo[1], hi[1]);
+            for (int q = 0; q < 4; ++q)
+              keep(t * 8 + q * 2 + g, make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]), __float_as_uint(v[4 * q + 3])));
+          } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const auto lo = __builtin_amdgcn_permlane32_swap(f32_to_bf16_pair(v[8 * h], v[8 * h + 1]), f32_to_bf16_pair(v[8 * h + 4], v[8 * h + 5]), false, false);
+              const auto hi = __builtin_amdgcn_permlane32_swap(f32_to_bf16_pair(v[8 * h + 2], v[8 * h + 3]), f32_to_bf16_pair(v[8 * h + 6], v[8 * h + 7]), false, false);
+              keep(t * 4 + h * 2 + g, make_uint4(lo[0], hi[0], lo[1], hi[1]));
+            }
           }
+        }
 #pragma unroll
-        for (int i = 0; i < 2 * NT; ++i) {
-          constexpr int P = 4 * NT;                 // pieces of a row
-          const int lrow = i * (64 / P) + lane / P, n = n_base + lane % P * 8;
-          const uint4 v = *reinterpret_cast<const uint4*>(mine + lrow * (64 * NT) + (lane % P ^ (lrow & (P - 1))) * 16);
-          if (first + lrow < row_end && n < o.n_out) *reinterpret_cast<uint4*>(o.out + (size_t)(first + lrow) * o.n_out + n) = v;
+        for (int i = 0; i < 32 * P / kWave; ++i) {
+          const int lrow = i * (kWave / P) + lane / P, n = n_base + lane % P * V;
+          const uint4 v = *reinterpret_cast<const uint4*>(mine + lrow * (P * 16) + (lane % P ^ (lrow & (P < 8 ? P - 1 : 7))) * 16);
+          if (first + lrow < row_end && n < o.n_out) *reinterpret_cast<uint4*>(out + (size_t)(first + lrow) * o.n_out + n) = v;
         }
       } else if (first + r < row_end) {
-        bf16_t* dst = o.out + (size_t)(first + r) * o.n_out;
+        TO* dst = out + (size_t)(first + r) * o.n_out;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int n = n_base + t * 32 + (i / 4) * 8 + g * 4 + i % 4;
-            if (n < o.n_out) dst[n] = f32_to_bf16(acc[t][m][i]);
+            if (n < o.n_out) dst[n] = from_f32<TO>(acc[t][m][i]);
           }
       }
     }
@@ -345,7 +354,7 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
 constexpr int kSideBySide = 4;
 constexpr int kDies = 8;
 
-template <int NT, bool GATED, bool PAIRED>
+template <int NT, bool GATED, bool PAIRED, typename TO = bf16_t>
 __global__ __launch_bounds__(TW* kWave, PAIRED ? 4 : 2) void fp8_tiles_kernel(F8Tiles p, F8Out o, GatedAct act) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[Ring<PAIRED>::kLds];
   __shared__ float s_top[GATED ? TWC : 1][64 * Ring<PAIRED>::kHighest];
@@ -411,7 +420,7 @@ __global__ __launch_bounds__(TW* kWave, PAIRED ? 4 : 2) void fp8_tiles_kernel(F8
   }
   const int rows = row_end - row0;
   if (rows <= 0) return;
-#define F8_TILE(MTV) f8_tile<MTV, NT, GATED, PAIRED>(p, o, act, e, row0, row_end, nblock, smem, s_top)
+#define F8_TILE(MTV) f8_tile<MTV, NT, GATED, PAIRED, TO>(p, o, act, e, row0, row_end, nblock, smem, s_top)
   if (rows <= 64) F8_TILE(1);
   else if (PAIRED || rows <= 128) F8_TILE(2);
   else if constexpr (!PAIRED) {
@@ -427,7 +436,7 @@ bool tiles_ok(const F8Tiles& p, int x_rows) {
          (!p.a_rows || (long long)x_rows * p.U * kF8Block <= 0xffffffffLL) && (long long)p.U * kF8TileBytes <= 0x7fffffffLL;
 }
 
-template <bool GATED> int launch_tiles(F8Tiles p, const F8Out& o, GatedAct act, int nt, hipStream_t stream) {
+template <bool GATED> int launch_tiles(F8Tiles p, const F8Out& o, GatedAct act, int nt, int dtype, hipStream_t stream) {
   const int height = p.height;
   if (height < 64 || height > 64 * Ring<false>::kHighest || height % 64) return SHARPI_ERR_ARG;
   const long long tiles = p.offsets ? (long long)p.rows / height + (p.rows < p.groups ? p.rows : p.groups) + (p.along + height - 1) / height
@@ -437,6 +446,16 @@ template <bool GATED> int launch_tiles(F8Tiles p, const F8Out& o, GatedAct act, 
   p.tiles = (int)tiles;
   if (tiles * p.nb > 0x7fffffffLL) return SHARPI_ERR_ARG;
   const dim3 grid((unsigned)(tiles * p.nb)), block(TW * kWave);
+  if constexpr (!GATED) {
+    if (dtype == DT_F32) {
+      if (nt != 2) return SHARPI_ERR_ARG;
+      if (height <= 64 * Ring<true>::kHighest) fp8_tiles_kernel<2, false, true, float><<<grid, block, 0, stream>>>(p, o, act);
+      else fp8_tiles_kernel<2, false, false, float><<<grid, block, 0, stream>>>(p, o, act);
+      SHARPI_CHECK_LAUNCH();
+      return SHARPI_OK;
+    }
+  }
+  if (dtype != DT_BF16) return SHARPI_ERR_ARG;
   if (height <= 64 * Ring<true>::kHighest) fp8_tiles_kernel<2, GATED, true><<<grid, block, 0, stream>>>(p, o, act);
   else if (nt == 2) fp8_tiles_kernel<2, GATED, false><<<grid, block, 0, stream>>>(p, o, act);
   else if constexpr (!GATED) fp8_tiles_kernel<1, GATED, false><<<grid, block, 0, stream>>>(p, o, act);
@@ -446,15 +465,15 @@ template <bool GATED> int launch_tiles(F8Tiles p, const F8Out& o, GatedAct act, 
 
 }  // namespace
 
-// out [rows, N] bfloat16.  x: codes [x_rows, 128 U] and scales; w_rows: stored rows of one matrix; a_rows, offsets: of a sorted row list, or null; along: rows
+// out [rows, N], dtype DT_BF16 (or DT_F32 with nt 2).  x: codes [x_rows, 128 U] and scales; w_rows: stored rows of one matrix; a_rows, offsets: of a sorted row list, or null; along: rows
 // behind the list's `rows`, which matrix `groups` takes (row i reads row i - rows of x if there is a_rows); height: rows of a tile at most (64, 128, 192, 256); nt: its columns, 128 nt (1 with heights from 192 on).
-SHARPI_EXPORT int sharpi_fp8_tiles(const void* x, const void* x_scales, int x_rows, const void* w_codes, const void* w_scales, int w_rows, void* out,
+SHARPI_EXPORT int sharpi_fp8_tiles(const void* x, const void* x_scales, int x_rows, const void* w_codes, const void* w_scales, int w_rows, void* out, int dtype,
                                    int rows, int N, int K, const int* a_rows, const int* offsets, int groups, int along, int height, int nt, hipStream_t stream) {
   if (rows <= 0) return SHARPI_OK;
   if (N <= 0 || K <= 0 || w_rows != f8_padded_rows(N)) return SHARPI_ERR_ARG;
   const F8Tiles p{(const uint8_t*)x, (const uint8_t*)x_scales, (const uint8_t*)w_codes, (const uint8_t*)w_scales, f8_blocks(K), w_rows, a_rows, offsets, rows, groups, (uint32_t)((long long)x_rows * f8_blocks(K) * kF8Block), along, height, 0, 0};
   if (!tiles_ok(p, x_rows)) return SHARPI_ERR_ARG;
-  return launch_tiles<false>(p, F8Out{(bf16_t*)out, nullptr, nullptr, nullptr, N}, GatedAct{}, nt, stream);
+  return launch_tiles<false>(p, F8Out{out, nullptr, nullptr, nullptr, N}, GatedAct{}, nt, dtype, stream);
 }
 
 // codes [rows, 128 f8_blocks(I)] and scales [rows, f8_scale_stride(I)] of act(s g) (s u); w_rows: twice I up to a multiple of 32; score [rows] or null.
@@ -466,5 +485,5 @@ SHARPI_EXPORT int sharpi_fp8_tiles_gated(const void* x, const void* x_scales, in
   if (I <= 0 || K <= 0 || w_rows != 2 * f8_padded_rows(I) || !act_known(ga) || ((uintptr_t)codes & 15)) return SHARPI_ERR_ARG;
   const F8Tiles p{(const uint8_t*)x, (const uint8_t*)x_scales, (const uint8_t*)w_codes, (const uint8_t*)w_scales, f8_blocks(K), w_rows, a_rows, offsets, rows, groups, (uint32_t)((long long)x_rows * f8_blocks(K) * kF8Block), along, height, 0, 0};
   if (!tiles_ok(p, x_rows)) return SHARPI_ERR_ARG;
-  return launch_tiles<true>(p, F8Out{nullptr, (uint8_t*)codes, (uint8_t*)scales, score, I}, ga, 2, stream);
+  return launch_tiles<true>(p, F8Out{nullptr, (uint8_t*)codes, (uint8_t*)scales, score, I}, ga, 2, DT_BF16, stream);
 }

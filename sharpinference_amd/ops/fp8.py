@@ -24,6 +24,7 @@ FP8_FEW_ROWS = 64              # rows of the weight-streaming kernels (csrc/fp8_
 FP8_FEW_PAIRS = 1024           # (token, pick) pairs of the same (kFewPairs)
 FP8_MAX_EXPERTS = 1023         # experts of a layer, one more may be always on (kFewExperts, kMaxGroups)
 FP8_STAGED_BYTES = 48 * 1024   # LDS for rows that are quantised where they are read (kStagedMost)
+_F32, _BF16 = _code(torch.float32), _code(torch.bfloat16)
 _X_CODES = 2                   # csrc/fp8_few.hip X_CODES
 
 
@@ -281,7 +282,7 @@ def linear_fp8(x: Union[torch.Tensor, Fp8Rows], w: Fp8Weight) -> torch.Tensor:
             _run("sharpi_fp8_few", a, scales, kind, w.codes.data_ptr(), w.scales.data_ptr(), w.stored_rows, out.data_ptr(), M, N, K,
                  _few_tiles(N), stream)
         else:
-            _run("sharpi_fp8_tiles", a, scales, M, w.codes.data_ptr(), w.scales.data_ptr(), w.stored_rows, out.data_ptr(), M, N, K,
+            _run("sharpi_fp8_tiles", a, scales, M, w.codes.data_ptr(), w.scales.data_ptr(), w.stored_rows, out.data_ptr(), _BF16, M, N, K,
                  None, None, 1, 0, *tile_fp8(M, N, K, False, compute_units()), stream)
     return out
 
@@ -359,10 +360,10 @@ def _few_layer(x, ids, wts, w1: Fp8Weight, w2: Fp8Weight, code: int, limit: floa
     w_in, w_out = (_ptr(wts), None) if on_input else (None, _ptr(wts))
     _run("sharpi_fp8_few_gated", a, scales, kind, w1.codes.data_ptr(), w1.scales.data_ptr(), w1.stored_rows, scratch[h], stride, ids_at, w_in,
          T, k, E, also, inner, K, code, limit, 2, scratch[counters], tiles, stream)
-    a, scales, kind = scratch[h], None, _code(torch.bfloat16)
+    a, scales, kind = scratch[h], None, _BF16
     if T > 16:
         a, scales, kind = scratch[codes], scratch[scales_at], _X_CODES
-        _run("sharpi_fp8_rows", scratch[h], _code(torch.bfloat16), a, scales, rows, stride, 0, 0.0, stream)
+        _run("sharpi_fp8_rows", scratch[h], _BF16, a, scales, rows, stride, 0, 0.0, stream)
     _run("sharpi_fp8_few_sum", a, scales, kind, w2.codes.data_ptr(), w2.scales.data_ptr(), w2.stored_rows, out.data_ptr(), ids_at, w_out, T, k, E,
          also, N, stride, SUM_TILES, shares, scratch[part], scratch[counters], stream)
     return out
@@ -396,7 +397,7 @@ def feed_forward_fp8(x: Union[torch.Tensor, Fp8Rows], w_gate_up: Fp8Weight, w_do
         _run("sharpi_fp8_tiles_gated", a, a_scales, M, w_gate_up.codes.data_ptr(), w_gate_up.scales.data_ptr(), w_gate_up.stored_rows, scratch[codes],
              scratch[scales], M, inner, K, None, None, 1, 0, None, code, limit, tile_fp8(M, inner, K, True, compute_units())[0], stream)
         _run("sharpi_fp8_tiles", scratch[codes], scratch[scales], M, w_down.codes.data_ptr(), w_down.scales.data_ptr(), w_down.stored_rows, out.data_ptr(),
-             M, N, inner, None, None, 1, 0, *tile_fp8(M, N, inner, False, compute_units()), stream)
+             _BF16, M, N, inner, None, None, 1, 0, *tile_fp8(M, N, inner, False, compute_units()), stream)
         return out
 
 
@@ -408,7 +409,7 @@ def experts_fp8(x: Union[torch.Tensor, Fp8Rows], ids: torch.Tensor, wts: torch.T
     gives them (``router_topk``); a pick of the experts' number or above adds nothing, negative ones are not allowed.  bfloat16 [T, N].
 
     Up to 64 tokens the picks are taken as they are: two launches for up to 16 rows of bfloat16 (four beyond), the second of which adds the experts' outputs in float.  More
-    tokens are sorted by expert; a pick's output is then rounded to bfloat16 before the sum."""
+    tokens are sorted by expert."""
     T, K, inner, N = _layer_checked(x, w_gate_up, w_down, 3, "experts_fp8")
     _dev(ids, wts)
     _i32(ids, "ids")
@@ -434,8 +435,8 @@ def _many_layer(x, ids, wts, w1: Fp8Weight, w2: Fp8Weight, code: int, limit: flo
     operand = _Operand(x, scratch, False)
     offsets, tokens, inv_pos, scores = scratch.add((E + 1) * 4), scratch.add(n * 4), scratch.add(n * 4), scratch.add(n * 4)
     codes, scales = scratch.add((n + along) * _blocks(inner) * FP8_BLOCK), scratch.add((n + along) * _scale_stride(inner))
-    y = scratch.add((n + along) * N * 2)
-    shared_y = y + n * N * 2
+    y = scratch.add((n + along) * N * 4)
+    shared_y = y + n * N * 4
     scratch.make(dev)
     out = torch.empty((T, N), dtype=torch.bfloat16, device=dev)
     stream, height = _stream_of(out), grouped_tile_fp8(n, E)
@@ -444,7 +445,7 @@ def _many_layer(x, ids, wts, w1: Fp8Weight, w2: Fp8Weight, code: int, limit: flo
          T, k, E, 0, 1, stream)
     _run("sharpi_fp8_tiles_gated", a, a_scales, T, w1.codes.data_ptr(), w1.scales.data_ptr(), w1.stored_rows, scratch[codes], scratch[scales],
          n, inner, w1.shape[-1], scratch[tokens], scratch[offsets], E, along, scratch[scores] if on_input else None, code, limit, height, stream)
-    _run("sharpi_fp8_tiles", scratch[codes], scratch[scales], n + along, w2.codes.data_ptr(), w2.scales.data_ptr(), w2.stored_rows, scratch[y], n, N, inner,
+    _run("sharpi_fp8_tiles", scratch[codes], scratch[scales], n + along, w2.codes.data_ptr(), w2.scales.data_ptr(), w2.stored_rows, scratch[y], _F32, n, N, inner,
          None, scratch[offsets], E, along, height, 2, stream)
     _run("sharpi_fp8_combine", scratch[y], scratch[inv_pos], ids.data_ptr(), scratch[shared_y] if shared else None, None if on_input else wts.data_ptr(),
          out.data_ptr(), T, N, k, E, stream)

@@ -219,7 +219,7 @@ def _layer_want(x, ids, wts, w1, w2, act, on_input, shared):
             y, d = plain.feed_forward(x[at].double(), a, b, act, s if on_input else None)
             f = s[:, None].double() if s is not None and not on_input else 1.0
             want[at] += y * f
-            bound[at] += (d + (plain.stored(y) if T > 64 else 0.0)) * f       # (many tokens: a pick's output is stored before the sum)
+            bound[at] += d * f
     return want, bound
 
 
