@@ -21,7 +21,7 @@ namespace {
 
 constexpr int FW = 8;                  // waves a block
 constexpr int kFewRows = 64;           // rows (tokens) of a call at most: four row blocks
-constexpr int kFewPairs = 1024;        // (token, pick) pairs of a call at most
+constexpr int kFewPairs = 512;         // (token, pick) pairs of a call at most
 constexpr int kFewExperts = 1024;
 constexpr int kRound = 2;              // (tile, row block) pairs that meet in LDS at a time
 
@@ -389,7 +389,7 @@ __global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_sum_kernel(cons
   static_assert(!STAGED || MB == 1, "staged rows are one row block");
   extern __shared__ __attribute__((aligned(16))) uint8_t staged_bytes[];
   __shared__ f32x4 red[FW][kRound][kWave];
-  __shared__ int ids[kFewPairs];
+  __shared__ short ids[kFewPairs];              // (-1: a pick of no expert)
   __shared__ float wts[kFewPairs];
   __shared__ int occurs[kFewExperts];           // times that one token picks the expert, at most
   __shared__ int entry[kFewPairs + 1];          // expert | occurrence << 16
@@ -399,7 +399,8 @@ __global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_sum_kernel(cons
   const int n_pairs = pk.ids ? pk.T * pk.k : 0;
   if (pk.ids) {
     for (int i = threadIdx.x; i < n_pairs; i += FW * kWave) {
-      ids[i] = pk.ids[i];
+      const int e = pk.ids[i];
+      ids[i] = (unsigned)e < (unsigned)pk.E ? (short)e : (short)-1;
       if (weighted) wts[i] = pk.w[i];
     }
     for (int i = threadIdx.x; i < pk.E; i += FW * kWave) occurs[i] = 0;
@@ -408,7 +409,7 @@ __global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_sum_kernel(cons
       const int e = ids[i];
       int n = 1;
       for (int j = i / pk.k * pk.k; j < i; ++j) n += ids[j] == e;
-      if ((unsigned)e < (unsigned)pk.E) atomicMax(&occurs[e], n);
+      if (e >= 0) atomicMax(&occurs[e], n);
     }
     __syncthreads();
     if (w == 0) {                               // (expert, occurrence) entries in the experts' order, the always-on one last

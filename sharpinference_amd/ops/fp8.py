@@ -21,8 +21,10 @@ from . import ACT_SILU, _code, _dev, _i32, _known_act_pair, _need, _ptr, _run, c
 FP8_BLOCK = 128                # values that share a scale
 FP8_TILE = 32                  # weight rows of a stored tile
 FP8_FEW_ROWS = 64              # rows of the weight-streaming kernels (csrc/fp8_few.hip kFewRows)
-FP8_FEW_PAIRS = 1024           # (token, pick) pairs of the same (kFewPairs)
+FP8_FEW_PAIRS = 512            # (token, pick) pairs of the same (kFewPairs)
 FP8_MAX_EXPERTS = 1023         # experts of a layer, one more may be always on (kFewExperts, kMaxGroups)
+FP8_STAGED_ROWS = 4
+FP8_STAGED_SUM = 2
 FP8_STAGED_BYTES = 48 * 1024   # LDS for rows that are quantised where they are read (kStagedMost)
 _F32, _BF16 = _code(torch.float32), _code(torch.bfloat16)
 _X_CODES = 2                   # csrc/fp8_few.hip X_CODES
@@ -223,8 +225,8 @@ def quantize_rows(x: torch.Tensor, act=None) -> Fp8Rows:
 
 
 def _staged(x) -> bool:
-    """Whether the weight-streaming kernels quantise these rows where they are read: up to 16 rows of bfloat16 that fit in LDS."""
-    return (isinstance(x, torch.Tensor) and x.dtype == torch.bfloat16 and x.shape[0] <= 16 and x.shape[1] % 8 == 0 and x.data_ptr() % 16 == 0
+    """Whether the weight-streaming kernels quantise these rows where they are read: a few rows of bfloat16 that fit in LDS."""
+    return (isinstance(x, torch.Tensor) and x.dtype == torch.bfloat16 and x.shape[0] <= FP8_STAGED_ROWS and x.shape[1] % 8 == 0 and x.data_ptr() % 16 == 0
             and x.shape[0] * _blocks(x.shape[1]) * (FP8_BLOCK + 1) + 16 <= FP8_STAGED_BYTES)
 
 
@@ -351,7 +353,7 @@ def _few_layer(x, ids, wts, w1: Fp8Weight, w2: Fp8Weight, code: int, limit: floa
     h, counters = scratch.add(rows * stride * 2), scratch.add(tiles * 4)
     part = scratch.add(shares * tiles * SUM_TILES * row_blocks * 1024 if shares > 1 else 0)
     operand = _Operand(x, scratch, _staged(x))
-    if T > 16:
+    if T > FP8_STAGED_SUM:
         codes, scales_at = scratch.add(rows * _blocks(stride) * FP8_BLOCK), scratch.add(rows * _scale_stride(stride))
     scratch.make(w1.codes.device)
     out = torch.empty((T, N), dtype=torch.bfloat16, device=w1.codes.device)
@@ -361,7 +363,7 @@ def _few_layer(x, ids, wts, w1: Fp8Weight, w2: Fp8Weight, code: int, limit: floa
     _run("sharpi_fp8_few_gated", a, scales, kind, w1.codes.data_ptr(), w1.scales.data_ptr(), w1.stored_rows, scratch[h], stride, ids_at, w_in,
          T, k, E, also, inner, K, code, limit, 2, scratch[counters], tiles, stream)
     a, scales, kind = scratch[h], None, _BF16
-    if T > 16:
+    if T > FP8_STAGED_SUM:
         a, scales, kind = scratch[codes], scratch[scales_at], _X_CODES
         _run("sharpi_fp8_rows", scratch[h], _BF16, a, scales, rows, stride, 0, 0.0, stream)
     _run("sharpi_fp8_few_sum", a, scales, kind, w2.codes.data_ptr(), w2.scales.data_ptr(), w2.stored_rows, out.data_ptr(), ids_at, w_out, T, k, E,
