@@ -126,3 +126,28 @@ SHARPI_EXPORT int sharpi_fp8_combine(const float* y, const int* inv_pos, const i
   SHARPI_CHECK_LAUNCH();
   return SHARPI_OK;
 }
+
+// out = the sum of `shares` arrays of n floats on end, in their order, rounded to bfloat16.  Bound: a pass over them.
+__global__ __launch_bounds__(256) void fp8_join_kernel(const float* __restrict__ part, bf16_t* __restrict__ out, long long n, int shares) {
+  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  if ((n & 3) == 0 && (((uintptr_t)part | (uintptr_t)out) & 15) == 0) {
+    f32x4 v = *reinterpret_cast<const f32x4*>(part + i);
+    for (int s = 1; s < shares; ++s) v += *reinterpret_cast<const f32x4*>(part + s * n + i);
+    *reinterpret_cast<uint2*>(out + i) = make_uint2(f32_to_bf16_pair(v[0], v[1]), f32_to_bf16_pair(v[2], v[3]));
+    return;
+  }
+  for (int j = 0; j < 4 && i + j < n; ++j) {
+    float v = part[i + j];
+    for (int s = 1; s < shares; ++s) v += part[s * n + i + j];
+    out[i + j] = f32_to_bf16(v);
+  }
+}
+
+SHARPI_EXPORT int sharpi_fp8_join(const float* part, void* out, long long n, int shares, hipStream_t stream) {
+  if (n <= 0) return SHARPI_OK;
+  if (shares < 1 || (n + 1023) / 1024 > 0x7fffffffLL) return SHARPI_ERR_ARG;
+  fp8_join_kernel<<<dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, stream>>>(part, (bf16_t*)out, n, shares);
+  SHARPI_CHECK_LAUNCH();
+  return SHARPI_OK;
+}

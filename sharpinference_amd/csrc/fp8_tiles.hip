@@ -30,6 +30,7 @@ struct F8Tiles {
   int along;                 // rows behind these that one more matrix takes, in the order of x (0: none)
   int height;                // rows of a tile at most, a multiple of 64
   int tiles, nb;             // row tiles in all at most; column blocks
+  int shares;                // of the blocks of k (plain form): share s of them gives row s * rows + row of the result
 };
 
 // plain: out [rows, n_out], bfloat16 or float.  gated: codes [rows, 128 f8_blocks(n_out)], scales [rows, f8_scale_stride(n_out)], score [rows] or null.
@@ -95,7 +96,8 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
     return !p.a_rows ? row - row0 : sorted ? p.a_rows[row] : row - p.rows;
   };
   constexpr int XL = (MT + 1) / 2;                        // loads of rows a wave and step (of 4 MT; some twice, to the same place)
-  const int steps = 2 * p.U;
+  // this block's steps of k (a share: whole blocks)
+  const int first_step = 2 * (int)((long long)p.U * blockIdx.y / gridDim.y), steps = 2 * (int)((long long)p.U * (blockIdx.y + 1) / gridDim.y);
   const uint32_t w_off[2] = {(uint32_t)lane * 16 + (NT == 1 ? (wid & 1) * 1024 : 0), (uint32_t)lane * 16 + 1024};
   auto load_w = [&](int s, uint32_t at) {                 // (past the end: the last step once more, for nobody)
     const uint32_t from = min(s, steps - 1) * 2048, to = lds0 + at + wid * (1024 * NT);
@@ -140,11 +142,12 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
     for (int i = 0; i < XL; ++i) to[i] = lds0 + at + x_to[i];
     bring_all_to_lds<true, XL>(xb, x_off, min(s, steps - 1) * 64, to);
   };
-  load_s(-1, true);
+  load_s((first_step >> 3) - 1, true);
+  load_s(first_step >> 3, true);                          // (the next chunk may begin a block further on)
 #pragma unroll
   for (int s = 0; s < AHEAD; ++s) {
-    load_w(s, s * kStep);
-    load_x(s, s * kStep);
+    load_w(first_step + s, s * kStep);
+    load_x(first_step + s, s * kStep);
   }
 
   f32x16 acc[NT][MT];
@@ -238,11 +241,11 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
   };
   lds_loads_wait<0>();
   __syncthreads();
-  read_scales(0, bw, bx);
+  read_scales(first_step >> 1, bw, bx);
   read_w(wf);
   read_rows(x0, 0, H0);
-  load_w(AHEAD, AHEAD * kStep);
-  for (int s = 0; s < steps; s += 2) {
+  load_w(first_step + AHEAD, AHEAD * kStep);
+  for (int s = first_step; s < steps; s += 2) {
     step(s, std::integral_constant<int, 0>{});
     step(s + 1, std::integral_constant<int, 1>{});
   }
@@ -255,8 +258,8 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
     // a lane first exchanges halves with lane ^ 32, so that it has eight columns of its row.  Rows that do not begin at 16-byte addresses are
     // stored by elements.  (Stored from the registers, pieces of 16 bytes a row, 8,192 x 2,048 x 2,560 in one round of tiles took 49 us, so 39.)
     constexpr int V = 16 / sizeof(TO), P = 32 * NT / V;      // columns of a 16-byte piece, pieces of a row
-    TO* out = (TO*)o.out;
-    const bool wide = o.n_out % V == 0 && ((uintptr_t)out & 15) == 0;
+    TO* out = (TO*)o.out + (size_t)blockIdx.y * p.rows * o.n_out;
+    const bool wide = o.n_out % V == 0 && ((uintptr_t)o.out & 15) == 0;
     __syncthreads();
     unsigned char* mine = smem + wid * (32 * P * 16);
 #pragma unroll
@@ -360,6 +363,7 @@ __global__ __launch_bounds__(TW* kWave, PAIRED ? 4 : 2) void fp8_tiles_kernel(F8
   __shared__ float s_top[GATED ? TWC : 1][64 * Ring<PAIRED>::kHighest];
   __shared__ int s_found[3];
   const int lane = threadIdx.x & (kWave - 1);
+  // (shares of k one after the other: gridDim.y)
   const int slots = gridDim.x, die = blockIdx.x % kDies;
   const int slot = die * (slots / kDies) + min(die, slots % kDies) + blockIdx.x / kDies;
   const int c0 = slot / (kSideBySide * p.tiles) * kSideBySide, left = slot - c0 * p.tiles, wide = min(kSideBySide, p.nb - c0);
@@ -445,11 +449,12 @@ template <bool GATED> int launch_tiles(F8Tiles p, const F8Out& o, GatedAct act, 
   p.nb = ceil_div(o.n_out, GATED ? columns_of(nt) / 2 : columns_of(nt));
   p.tiles = (int)tiles;
   if (tiles * p.nb > 0x7fffffffLL) return SHARPI_ERR_ARG;
-  const dim3 grid((unsigned)(tiles * p.nb)), block(TW * kWave);
+  if (p.shares < 1 || p.shares > p.U || (p.shares > 1 && (GATED || p.offsets || dtype != DT_F32))) return SHARPI_ERR_ARG;
+  const dim3 grid((unsigned)(tiles * p.nb), (unsigned)p.shares), block(TW * kWave);
   if constexpr (!GATED) {
     if (dtype == DT_F32) {
-      if (nt != 2) return SHARPI_ERR_ARG;
       if (height <= 64 * Ring<true>::kHighest) fp8_tiles_kernel<2, false, true, float><<<grid, block, 0, stream>>>(p, o, act);
+      else if (nt == 1) fp8_tiles_kernel<1, false, false, float><<<grid, block, 0, stream>>>(p, o, act);
       else fp8_tiles_kernel<2, false, false, float><<<grid, block, 0, stream>>>(p, o, act);
       SHARPI_CHECK_LAUNCH();
       return SHARPI_OK;
@@ -465,13 +470,14 @@ template <bool GATED> int launch_tiles(F8Tiles p, const F8Out& o, GatedAct act, 
 
 }  // namespace
 
-// out [rows, N], dtype DT_BF16 (or DT_F32 with nt 2).  x: codes [x_rows, 128 U] and scales; w_rows: stored rows of one matrix; a_rows, offsets: of a sorted row list, or null; along: rows
+// out [rows, N], dtype DT_BF16 or DT_F32; with shares > 1 (DT_F32, one matrix) [shares, rows, N] to be added up.  x: codes [x_rows, 128 U] and scales; w_rows: stored rows of one matrix; a_rows, offsets: of a sorted row list, or null; along: rows
 // behind the list's `rows`, which matrix `groups` takes (row i reads row i - rows of x if there is a_rows); height: rows of a tile at most (64, 128, 192, 256); nt: its columns, 128 nt (1 with heights from 192 on).
 SHARPI_EXPORT int sharpi_fp8_tiles(const void* x, const void* x_scales, int x_rows, const void* w_codes, const void* w_scales, int w_rows, void* out, int dtype,
-                                   int rows, int N, int K, const int* a_rows, const int* offsets, int groups, int along, int height, int nt, hipStream_t stream) {
+                                   int rows, int N, int K, const int* a_rows, const int* offsets, int groups, int along, int height, int nt, int shares,
+                                   hipStream_t stream) {
   if (rows <= 0) return SHARPI_OK;
   if (N <= 0 || K <= 0 || w_rows != f8_padded_rows(N)) return SHARPI_ERR_ARG;
-  const F8Tiles p{(const uint8_t*)x, (const uint8_t*)x_scales, (const uint8_t*)w_codes, (const uint8_t*)w_scales, f8_blocks(K), w_rows, a_rows, offsets, rows, groups, (uint32_t)((long long)x_rows * f8_blocks(K) * kF8Block), along, height, 0, 0};
+  const F8Tiles p{(const uint8_t*)x, (const uint8_t*)x_scales, (const uint8_t*)w_codes, (const uint8_t*)w_scales, f8_blocks(K), w_rows, a_rows, offsets, rows, groups, (uint32_t)((long long)x_rows * f8_blocks(K) * kF8Block), along, height, 0, 0, shares};
   if (!tiles_ok(p, x_rows)) return SHARPI_ERR_ARG;
   return launch_tiles<false>(p, F8Out{out, nullptr, nullptr, nullptr, N}, GatedAct{}, nt, dtype, stream);
 }
@@ -483,7 +489,7 @@ SHARPI_EXPORT int sharpi_fp8_tiles_gated(const void* x, const void* x_scales, in
   if (rows <= 0) return SHARPI_OK;
   const GatedAct ga{act, limit};
   if (I <= 0 || K <= 0 || w_rows != 2 * f8_padded_rows(I) || !act_known(ga) || ((uintptr_t)codes & 15)) return SHARPI_ERR_ARG;
-  const F8Tiles p{(const uint8_t*)x, (const uint8_t*)x_scales, (const uint8_t*)w_codes, (const uint8_t*)w_scales, f8_blocks(K), w_rows, a_rows, offsets, rows, groups, (uint32_t)((long long)x_rows * f8_blocks(K) * kF8Block), along, height, 0, 0};
+  const F8Tiles p{(const uint8_t*)x, (const uint8_t*)x_scales, (const uint8_t*)w_codes, (const uint8_t*)w_scales, f8_blocks(K), w_rows, a_rows, offsets, rows, groups, (uint32_t)((long long)x_rows * f8_blocks(K) * kF8Block), along, height, 0, 0, 1};
   if (!tiles_ok(p, x_rows)) return SHARPI_ERR_ARG;
   return launch_tiles<true>(p, F8Out{nullptr, (uint8_t*)codes, (uint8_t*)scales, score, I}, ga, 2, DT_BF16, stream);
 }

@@ -11,7 +11,6 @@ from __future__ import annotations
 
 import contextlib
 import functools
-import math
 from typing import Optional, Tuple, Union
 
 import torch
@@ -21,6 +20,7 @@ from . import ACT_SILU, _code, _dev, _i32, _known_act_pair, _need, _ptr, _run, c
 FP8_BLOCK = 128                # values that share a scale
 FP8_TILE = 32                  # weight rows of a stored tile
 FP8_FEW_ROWS = 64              # rows of the weight-streaming kernels (csrc/fp8_few.hip kFewRows)
+FP8_FEW_TOKENS = 16            # tokens of a layer that takes the picks as they are
 FP8_FEW_PAIRS = 512            # (token, pick) pairs of the same (kFewPairs)
 FP8_MAX_EXPERTS = 1023         # experts of a layer, one more may be always on (kFewExperts, kMaxGroups)
 FP8_STAGED_ROWS = 4
@@ -275,6 +275,7 @@ def linear_fp8(x: Union[torch.Tensor, Fp8Rows], w: Fp8Weight) -> torch.Tensor:
     few = few_rows_fp8(M, N)
     scratch = _Scratch()
     rows = _Operand(x, scratch, few and _staged(x))
+    product = None if few else _Tiled(M, N, K, scratch)
     if scratch.size:
         scratch.make(out.device)
     with _device_of(out):
@@ -284,19 +285,42 @@ def linear_fp8(x: Union[torch.Tensor, Fp8Rows], w: Fp8Weight) -> torch.Tensor:
             _run("sharpi_fp8_few", a, scales, kind, w.codes.data_ptr(), w.scales.data_ptr(), w.stored_rows, out.data_ptr(), M, N, K,
                  _few_tiles(N), stream)
         else:
-            _run("sharpi_fp8_tiles", a, scales, M, w.codes.data_ptr(), w.scales.data_ptr(), w.stored_rows, out.data_ptr(), _BF16, M, N, K,
-                 None, None, 1, 0, *tile_fp8(M, N, K, False, compute_units()), stream)
+            product.run(a, scales, w, out, scratch, stream)
     return out
 
 
+class _Tiled:
+    """A product of many rows by one matrix in tiles; where these are few, shares of k go side by side and are added up behind them."""
+
+    __slots__ = ("shape", "height", "nt", "shares", "part_at")
+
+    def __init__(self, M: int, N: int, K: int, scratch: _Scratch):
+        self.shape = (M, N, K)
+        self.height, self.nt, self.shares = tile_fp8(M, N, K, False, compute_units())
+        if self.shares > 1:
+            self.part_at = scratch.add(self.shares * M * N * 4)
+
+    def run(self, codes: int, scales: int, w: Fp8Weight, out: torch.Tensor, scratch: _Scratch, stream: int) -> None:
+        M, N, K = self.shape
+        whole = self.shares == 1
+        to = out.data_ptr() if whole else scratch[self.part_at]
+        _run("sharpi_fp8_tiles", codes, scales, M, w.codes.data_ptr(), w.scales.data_ptr(), w.stored_rows, to, _BF16 if whole else _F32, M, N, K,
+             None, None, 1, 0, self.height, self.nt, self.shares, stream)
+        if not whole:
+            _run("sharpi_fp8_join", to, out.data_ptr(), M * N, self.shares, stream)
+
+
 def few_rows_fp8(M: int, N: int) -> bool:
-    """Whether a product of M rows goes by streaming the weights."""
-    return M <= FP8_FEW_ROWS
+    """Whether a product of M rows goes by streaming the weights: up to 16 rows always; then while the rows' blocks of 16 times the columns are few (us,
+    streamed and in tiles, K 5,120: 7,168 columns 48 rows 19 and 30, 64 rows 22 and 31; 16,384 columns 32 rows 27 and 33, 64 rows 38 and 36; 65,536 columns 16
+    rows 62 and 71, 24 rows 82 and 66)."""
+    return M <= 16 or (M <= FP8_FEW_ROWS and -(-M // 16) * N <= 49152)
 
 
 def _few_tiles(N: int) -> int:
-    """Half tiles of 16 weight rows a block takes."""
-    return 2 if N >= 16384 else 1
+    """Half tiles of 16 weight rows a block takes: two where that leaves blocks for half of the compute units (us, one and two, 16 rows: 5,120 x 5,120 14.1
+    and 11.8, 65,536 x 5,120 85 and 62, 4,096 x 14,336 19.4 and 23.5, 1,024 x 2,048 7.0 and 7.6)."""
+    return 2 if N >= 4608 else 1
 
 
 # us that a step of 64 of k takes in a tile, where it runs alone on the chip and where all compute units do, by (rows / 64, columns / 128); tiles of up to 128
@@ -306,28 +330,33 @@ PAIRED_STEP_US = {1: (0.38, 0.62), 2: (0.42, 0.86)}
 TILE_END_US = 5.0
 
 
-@functools.lru_cache(maxsize=1024)
-def tile_fp8(M: int, N: int, K: int, gated: bool, units: int) -> Tuple[int, int]:
-    """(rows, columns / 128) of the tiles of a product of many rows (gated: 256 columns): those whose rounds of the chip take the least time."""
-    steps = 2 * _blocks(K)
+JOIN_US, JOIN_TBS = 3.0, 6.0      # adding shares up: a launch, and the rate at which they are written and read again
 
-    def expected(height: int, nt: int) -> float:
-        blocks = -(-M // height) * -(-N // (128 if gated else 128 * nt))
+
+@functools.lru_cache(maxsize=1024)
+def tile_fp8(M: int, N: int, K: int, gated: bool, units: int) -> Tuple[int, int, int]:
+    """(rows, columns / 128, shares of k) of the tiles of a product of many rows (gated: 256 columns, one share): those whose rounds of the chip take the
+    least time."""
+    def expected(height: int, nt: int, shares: int) -> float:
+        steps = 2 * -(-_blocks(K) // shares)
+        blocks = -(-M // height) * -(-N // (128 if gated else 128 * nt)) * shares
         tall = -(-min(M, height) // 64)
         low, full = PAIRED_STEP_US[tall] if height <= 128 else TILE_STEP_US[(tall, nt)] if (tall, nt) in TILE_STEP_US else TILE_STEP_US[(3, nt)]
         at_once = 2 * units if height <= 128 else units
         rounds, rest = divmod(blocks, at_once)
         us = rounds * (full * steps + TILE_END_US)
         if rest:
-            fill = max(0.0, (rest - units) / units) if height <= 128 else rest / units
+            fill = float(rest > units) if height <= 128 else rest / units        # (a unit with a pair takes as long as all of them)
             us += (low + (full - low) * fill) * steps + TILE_END_US
-        return us
+        return us + (JOIN_US + 8e-6 * shares * M * N / JOIN_TBS if shares > 1 else 0.0)
     choices = [(64, 2), (128, 2), (192, 2), (256, 2)] + ([] if gated else [(192, 1), (256, 1)])
-    return min(choices, key=lambda c: expected(*c))
+    most = 1 if gated else min(8, max(1, _blocks(K) // 4))
+    return min(((h, nt, s) for h, nt in choices for s in range(1, most + 1)), key=lambda c: expected(*c))
 
 
 def grouped_tile_fp8(rows: int, groups: int) -> int:
-    """Rows of the tiles of a layer's products at most."""
+    """Rows of the tiles of a layer's products at most: in pairs of blocks a unit where an expert has few (us, tiles of 128 and of 256: 64 experts of 2 x 1,408 x
+    2,048, 94 rows each 118 and 123; 16 of 5,120 x 8,192, 6 rows each 125 and 139, 128 rows each 223 and 205, their first product 357 and 326)."""
     return 128 if rows <= 96 * groups else 256
 
 
@@ -392,14 +421,14 @@ def feed_forward_fp8(x: Union[torch.Tensor, Fp8Rows], w_gate_up: Fp8Weight, w_do
         scratch = _Scratch()
         operand = _Operand(x, scratch, False)
         codes, scales = scratch.add(M * _blocks(inner) * FP8_BLOCK), scratch.add(M * _scale_stride(inner))
+        down = _Tiled(M, N, inner, scratch)
         scratch.make(w_down.codes.device)
         out = torch.empty((M, N), dtype=torch.bfloat16, device=w_down.codes.device)
         stream = _stream_of(out)
         a, a_scales, _ = operand.ready(scratch, stream)
         _run("sharpi_fp8_tiles_gated", a, a_scales, M, w_gate_up.codes.data_ptr(), w_gate_up.scales.data_ptr(), w_gate_up.stored_rows, scratch[codes],
              scratch[scales], M, inner, K, None, None, 1, 0, None, code, limit, tile_fp8(M, inner, K, True, compute_units())[0], stream)
-        _run("sharpi_fp8_tiles", scratch[codes], scratch[scales], M, w_down.codes.data_ptr(), w_down.scales.data_ptr(), w_down.stored_rows, out.data_ptr(),
-             _BF16, M, N, inner, None, None, 1, 0, *tile_fp8(M, N, inner, False, compute_units()), stream)
+        down.run(scratch[codes], scratch[scales], w_down, out, scratch, stream)
         return out
 
 
@@ -424,7 +453,7 @@ def experts_fp8(x: Union[torch.Tensor, Fp8Rows], ids: torch.Tensor, wts: torch.T
     with _device_of(w_down.codes):
         if T == 0:
             return torch.empty(0, N, dtype=torch.bfloat16, device=w_down.device)
-        if T <= FP8_FEW_ROWS and T * k <= FP8_FEW_PAIRS:
+        if T <= FP8_FEW_TOKENS and T * k <= FP8_FEW_PAIRS:
             return _few_layer(x, ids, wts, w_gate_up, w_down, code, limit, score_on_input, shared, E)
         return _many_layer(x, ids, wts, w_gate_up, w_down, code, limit, score_on_input, shared, E, inner, N)
 
@@ -448,7 +477,7 @@ def _many_layer(x, ids, wts, w1: Fp8Weight, w2: Fp8Weight, code: int, limit: flo
     _run("sharpi_fp8_tiles_gated", a, a_scales, T, w1.codes.data_ptr(), w1.scales.data_ptr(), w1.stored_rows, scratch[codes], scratch[scales],
          n, inner, w1.shape[-1], scratch[tokens], scratch[offsets], E, along, scratch[scores] if on_input else None, code, limit, height, stream)
     _run("sharpi_fp8_tiles", scratch[codes], scratch[scales], n + along, w2.codes.data_ptr(), w2.scales.data_ptr(), w2.stored_rows, scratch[y], _F32, n, N, inner,
-         None, scratch[offsets], E, along, height, 2, stream)
+         None, scratch[offsets], E, along, height, 2, 1, stream)
     _run("sharpi_fp8_combine", scratch[y], scratch[inv_pos], ids.data_ptr(), scratch[shared_y] if shared else None, None if on_input else wts.data_ptr(),
          out.data_ptr(), T, N, k, E, stream)
     return out

@@ -37,8 +37,9 @@ _SIGNATURES = {
     "sharpi_fp8_few": [P, P, I, P, P, I, P, I, I, I, I, P],
     "sharpi_fp8_few_gated": [P, P, I, P, P, I, P, I, P, P, I, I, I, I, I, I, I, F, I, P, I, P],
     "sharpi_fp8_few_sum": [P, P, I, P, P, I, P, P, P, I, I, I, I, I, I, I, I, P, P, P],
-    "sharpi_fp8_tiles": [P, P, I, P, P, I, P, I, I, I, I, P, P, I, I, I, I, P],
+    "sharpi_fp8_tiles": [P, P, I, P, P, I, P, I, I, I, I, P, P, I, I, I, I, I, P],
     "sharpi_fp8_tiles_gated": [P, P, I, P, P, I, P, P, I, I, I, P, P, I, I, P, I, F, I, P],
+    "sharpi_fp8_join": [P, P, c_longlong, I, P],
     "sharpi_fp8_combine": [P, P, P, P, P, P, I, I, I, I, P],
     "sharpi_gemm_tiled": [P, P, P, I, I, I, I, I, P, P, I, I, P],
     "sharpi_gemm_skinny": [P, P, P, I, I, I, I, P, P, I, I, I, I, I, I, P],
