@@ -107,6 +107,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--backend", default="auto", choices=["auto", "hip"], help="there is one backend: HIP on gfx950")
     # this engine's own
     ap.add_argument("--dtype", default="bf16", choices=["bf16", "fp32", "bfloat16", "float32"])
+    ap.add_argument("--feed-forward", default="bf16", choices=["bf16", "fp8"],
+                    help="how gated feed-forwards keep their matrices: as stored, or in 8-bit floating point (with --dtype bf16)")
     ap.add_argument("--random-weights", action="store_true", help="seeded random weights (folder needs config.json only)")
     ap.add_argument("--weight-seed", type=int, default=0)
     ap.add_argument("--parallel", type=int, default=1, help="generate this many copies of the prompt at once")
@@ -151,7 +153,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     ctx = args.ctx_size or None
     common = dict(dtype=dtype, device=device, max_model_len=ctx, max_num_seqs=max(args.max_num_seqs, args.parallel),
                   max_tokens_per_step=args.max_tokens_per_step, kv_tokens=args.kv_tokens, page_size=args.page_size,
-                  decode_graphs=not args.profile)
+                  decode_graphs=not args.profile, feed_forward={"bf16": "bfloat16"}.get(args.feed_forward, args.feed_forward))
     if args.random_weights:
         eng = Engine(config=cfg, weight_seed=args.weight_seed, **common)
     else:

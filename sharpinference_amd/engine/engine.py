@@ -70,13 +70,16 @@ class Engine:
                  kv_tokens: Optional[int] = None, page_size: int = 16, weight_std: float = 0.02,
                  weight_std_by_suffix: Optional[Dict[str, float]] = None, verbose: bool = False,
                  decode_graphs: bool = True, past_position_limit: bool = False, row_major_copies: bool = True,
-                 decode_run_ahead: int = 4):
+                 decode_run_ahead: int = 4, feed_forward: str = "bfloat16"):
         """max_model_len: the longest sequence a request may reach (default: the configuration's
         max_position_embeddings, 4096 if it names none); beyond max_position_embeddings only with
         past_position_limit (replaying given tokens needs no trained positions).
         row_major_copies=False keeps the attention, dense feed-forward and head matrices only in
         the packed order of the decode kernels (about a tenth less weight memory; prompt-sized
         products then run in this library's own kernels instead of the library product, slower).
+        feed_forward="fp8" keeps the matrices of gated feed-forwards, dense (without biases) and routed, in 8-bit
+        floating point with a power of two for each row's 128 values, and multiplies them by activations quantised
+        the same way (half of the weight bytes a decode step reads there, twice the matrix cores' rate; bfloat16 engines only).
         decode_run_ahead: while every running request decodes greedily and none waits, generation
         launches this many steps on end, each on what the step before chose (on the device), and
         reads the tokens back together: the host's part of a step then passes while the GPU works
@@ -84,6 +87,10 @@ class Engine:
         self.decode_run_ahead = max(1, int(decode_run_ahead))
         self.dtype = parse_dtype(dtype)
         self.device = torch.device(device)
+        if feed_forward not in ("bfloat16", "fp8"):
+            raise ValueError(f"feed_forward {feed_forward!r} is not known (bfloat16, fp8)")
+        if feed_forward == "fp8" and self.dtype != torch.bfloat16:
+            raise ValueError("feed_forward='fp8' belongs to a bfloat16 engine")
         if self.device.type != "cuda":
             raise RuntimeError("the engine runs on the GPU only (device must be cuda:N)")
         if not torch.cuda.is_available():
@@ -115,10 +122,12 @@ class Engine:
         from .. import ops as _ops
 
         _ops.keep_row_major_copies(row_major_copies)
+        _ops.feed_forwards_in_8_bits(feed_forward == "fp8")
         try:
             load_model_weights(self.model, source)
         finally:
             _ops.keep_row_major_copies(True)
+            _ops.feed_forwards_in_8_bits(False)
         if verbose:
             print(f"[engine] weights ready in {time.time() - t0:.1f}s", file=sys.stderr, flush=True)
         limit = getattr(self.config, "max_position_embeddings", 0) or 0

@@ -164,9 +164,9 @@ def _pack(codes: torch.Tensor, scales: torch.Tensor, gated: bool, dst_codes: tor
 
 
 def _new_weight(shape, gated: bool, device) -> Fp8Weight:
-    N, K = shape[-2:]
-    _need(len(shape) in (2, 3) and N > 0 and K > 0 and (len(shape) == 2 or 0 < shape[0] <= FP8_MAX_EXPERTS + 1),
+    _need(len(shape) in (2, 3) and min(shape) > 0 and (len(shape) == 2 or shape[0] <= FP8_MAX_EXPERTS + 1),
           f"8-bit weights must be [N, K] or [E, N, K] with at most {FP8_MAX_EXPERTS + 1} matrices")
+    N, K = shape[-2:]
     _need(not gated or N % 2 == 0, "a gated matrix holds gate rows, then as many up rows")
     R = 2 * _padded(N // 2) if gated else _padded(N)
     _need(R * _blocks(K) <= 0x7fffffff, f"8-bit weights [{N}, {K}] are too large")
@@ -190,15 +190,43 @@ def fp8_weight(codes: torch.Tensor, scales: torch.Tensor, gated: bool = False) -
     return w
 
 
+def empty_fp8_weight(shape, gated: bool, device) -> Fp8Weight:
+    """Room for a matrix [N, K] or a stack [E, N, K], to be filled by ``quantize_into`` (its own or ``select(e)``)."""
+    return _new_weight(tuple(int(n) for n in shape), gated, device)
+
+
+def quantize_into(dst: Fp8Weight, w: torch.Tensor) -> None:
+    """A bfloat16 or float32 matrix on the GPU, quantised (``quantize_rows`` of its rows) into dst [N, K] of its shape."""
+    _need(dst.dim() == 2 and tuple(w.shape) == dst.shape and w.device == dst.device, f"quantize_into: a matrix {dst.shape} on the destination's device is wanted")
+    q = quantize_rows(w.contiguous())
+    K = w.shape[1]
+    _pack(q.codes.view(torch.uint8)[:, :K], q.scales[:, :_blocks(K)], dst.gated, dst.codes, dst.scales)
+
+
 def quantize_weight(w: torch.Tensor, gated: bool = False) -> Fp8Weight:
-    """A bfloat16 or float32 matrix [(E,) N, K] on the GPU in 8 bits (``quantize_rows`` of its rows), in the kernels' order."""
+    """A bfloat16 or float32 matrix [(E,) N, K] on the GPU in 8 bits, in the kernels' order."""
     _need(w.is_cuda and w.dim() in (2, 3), "quantize_weight: a matrix [N, K] or a stack [E, N, K] on the GPU")
     out = _new_weight(tuple(w.shape), gated, w.device)
-    for e in range(w.shape[0] if w.dim() == 3 else 1):
-        q = quantize_rows((w[e] if w.dim() == 3 else w).contiguous())
-        codes, scales = q.codes.view(torch.uint8)[:, :w.shape[-1]], q.scales[:, :_blocks(w.shape[-1])]
-        _pack(codes, scales, gated, out.codes[e] if w.dim() == 3 else out.codes, out.scales[e] if w.dim() == 3 else out.scales)
+    if w.dim() == 2:
+        quantize_into(out, w)
+    else:
+        for e in range(w.shape[0]):
+            quantize_into(out.select(e), w[e])
     return out
+
+
+_FEED_FORWARDS = False
+
+
+def feed_forwards_in_8_bits(on: bool) -> None:
+    """Whether gated feed-forwards, dense and routed, keep bfloat16 matrices in 8 bits (half of the bytes of a decode step's largest reads) and run
+    through ``feed_forward_fp8`` and ``experts_fp8``.  Read when weights are loaded."""
+    global _FEED_FORWARDS
+    _FEED_FORWARDS = bool(on)
+
+
+def feed_forwards_are_8_bits() -> bool:
+    return _FEED_FORWARDS
 
 
 def _new_rows(M: int, k: int, device) -> Fp8Rows:

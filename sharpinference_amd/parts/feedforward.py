@@ -40,7 +40,10 @@ class DenseSwiGLU(Part):
     g = min(gate x, limit), u = clamp(up x, -limit, limit), and the unit is g sigmoid(1.702 g) (u + 1).  ``bias``: the three
     products carry biases (``names`` + ``bias_suffix``), added in float: the gate's and the up
     projection's inside the activation kernel, the down projection's by a row kernel.  ``names``:
-    the three matrices' names behind the part's prefix."""
+    the three matrices' names behind the part's prefix.
+
+    Loaded under ``ops.feed_forwards_in_8_bits`` bfloat16 matrices without biases are kept in 8 bits and the whole unit is
+    ``ops.feed_forward_fp8``."""
 
     NAMES = {"gate": "gate_proj.weight", "up": "up_proj.weight", "down": "down_proj.weight"}
 
@@ -72,6 +75,11 @@ class DenseSwiGLU(Part):
         n = self.names
         g = source.get(prefix + n["gate"])
         u = source.get(prefix + n["up"])
+        if ops.feed_forwards_are_8_bits() and not self.bias and g.dtype == u.dtype == torch.bfloat16:
+            self.w_gate_up = ops.quantize_weight(_fuse_rows(g, u), gated=True)
+            del g, u
+            self.w_down = ops.quantize_weight(source.get(prefix + n["down"]))
+            return
         # both also in the order the few-rows kernel streams them; the rows stay for prompt-sized steps
         self.w_gate_up = ops.pack_weight(_fuse_rows(g, u))
         del g, u
@@ -83,6 +91,10 @@ class DenseSwiGLU(Part):
     def forward(self, x: torch.Tensor, ctx: StepContext) -> torch.Tensor:
         T = x.shape[0]
         width = 2 if ctx.act_dtype == torch.bfloat16 else 4
+        if isinstance(self.w_gate_up, ops.Fp8Weight):
+            with section("dense feed-forward", nbytes=3 * self.inter * self.hidden + T * (4 * self.hidden + 4 * self.inter),
+                         flops=6.0 * T * self.inter * self.hidden):
+                return ops.feed_forward_fp8(x, self.w_gate_up, self.w_down, self.act)
         with section("dense feed-forward", nbytes=width * 3 * self.inter * self.hidden + width * T * (2 * self.hidden + 3 * self.inter),
                      flops=6.0 * T * self.inter * self.hidden):
             if self.b_gate_up is None:
@@ -142,7 +154,10 @@ class MoESwiGLU(Part):
     ``gated=False``: experts (and the shared one) without a gate, down( act(up x) ) with ``activation`` one of the
     ungated ones; no ``gate`` tensors.  ``identity`` n: the router scores n more experts behind the E there are, which
     have no tensors and return the layer's input; they take part in the choice (groups, correction) like the others.
-    Their share is added where the outputs are summed (``ops.ExpertSum``)."""
+    Their share is added where the outputs are summed (``ops.ExpertSum``).
+
+    Loaded under ``ops.feed_forwards_in_8_bits`` gated experts without identity experts beside them, of bfloat16 matrices, are kept
+    in 8 bits and run through ``ops.experts_fp8``, a shared expert of their width and activation as one more matrix."""
 
     MERGE_MAX_TOKENS = 16   # one row block of the few-rows kernel for the shared group (measured: up to 64 tokens
                             # the merged launches and the library's product for the shared expert are as fast)
@@ -260,6 +275,9 @@ class MoESwiGLU(Part):
         # The experts' matrices are kept only in the order the kernels stream them (no rows: both
         # the few-rows and the many-rows product of the experts read that order), if the sizes allow.
         pack = bf16 and self.inter % 128 == 0 and self.hidden % 128 == 0
+        if bf16 and self.gated and not self.identity and ops.feed_forwards_are_8_bits():
+            self._load_8_bits(g, u, d)
+            return
         sh_first = None if sh is None else "w_gate_up" if self.gated else "w_up"       # the shared expert's first matrix
         merge = (bf16 and sh is not None and sh.inter == self.inter and (not self.gated or sh.act == self.act)
                  and getattr(sh, sh_first).dtype == torch.bfloat16
@@ -295,12 +313,40 @@ class MoESwiGLU(Part):
         self.w_gate_up = ops.PackedWeight(gu, None) if pack else gu
         self.w_down = ops.PackedWeight(dn, None) if pack else dn
 
+    def _load_8_bits(self, g: torch.Tensor, u: torch.Tensor, d: torch.Tensor) -> None:
+        sh = self.shared
+        self.merged = (sh is not None and sh.inter == self.inter and sh.act == self.act and isinstance(sh.w_gate_up, ops.Fp8Weight)
+                       and isinstance(sh.w_down, ops.Fp8Weight))
+        n = self.E + (1 if self.merged else 0)
+        self.w_gate_up = ops.empty_fp8_weight((n, 2 * self.inter, self.hidden), True, u.device)
+        self.w_down = ops.empty_fp8_weight((n, self.hidden, self.inter), False, d.device)
+        for e in range(self.E):
+            ops.quantize_into(self.w_gate_up.select(e), _fuse_rows(g[e], u[e]))
+            ops.quantize_into(self.w_down.select(e), d[e])
+        if self.merged:
+            for name in ("w_gate_up", "w_down"):       # the shared expert's own copies give way to views of the stack
+                own = getattr(self, name).select(self.E)
+                own.codes.copy_(getattr(sh, name).codes)
+                own.scales.copy_(getattr(sh, name).scales)
+                setattr(sh, name, own)
+
+    def _8_bits(self, x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, ctx: StepContext):
+        """The experts (and the shared one, if it is a matrix of their stack) in 8 bits, summed."""
+        T = x.shape[0]
+        trace = ctx.extras.get("router_trace")
+        if trace is not None:      # the picks of this step, layer by layer (reference: ForwardPass.cs:2042-2056)
+            trace.append((ids, wts, x))
+        shared = None if self.merged or self.shared is None else self.shared.forward(x, ctx)
+        with self._experts_section(ids, T, self.merged):
+            y = ops.experts_fp8(x, ids, wts, self.w_gate_up, self.w_down, self.act, self.score_on_input, self.merged)
+        return y if shared is None else ops.ExpertSum(y, ops.counting(T, x.device), shared, T, 1)
+
     def _experts_section(self, ids: torch.Tensor, T: int, with_shared: bool):
         """The profiler's span of the experts' two products: every expert that a token picked is
         read once (the count is taken from the picks, only while profiling)."""
         if not profiling():
             return section("experts")
-        width = 2 if self.w_gate_up.dtype == torch.bfloat16 else 4
+        width = 1 if isinstance(self.w_gate_up, ops.Fp8Weight) else 2 if self.w_gate_up.dtype == torch.bfloat16 else 4
         own = ids[ids < self.E]                           # (identity experts multiply nothing)
         used = int(own.unique().numel()) + (1 if with_shared else 0)
         rows = int(own.numel()) + (T if with_shared else 0)
@@ -311,6 +357,8 @@ class MoESwiGLU(Part):
     def _few_tokens(self, T: int, ctx: StepContext) -> bool:
         """A few decode tokens in bfloat16 (at most 64 picks): the experts' two products find their
         rows from the picks themselves."""
+        if isinstance(self.w_gate_up, ops.Fp8Weight):
+            return T <= ops.FP8_FEW_TOKENS
         packed = isinstance(self.w_gate_up, ops.PackedWeight)
         return (ctx.act_dtype == torch.bfloat16 and self.w_gate_up.dtype == torch.bfloat16
                 and ops.picked_ok(T, self.k, (2 if self.gated else 1) * self.inter, self.hidden, self.gated, packed)
@@ -320,6 +368,8 @@ class MoESwiGLU(Part):
         """No sorting kernel: pair by pair in the picks' own order.  With up to MERGE_MAX_TOKENS
         tokens the shared expert rides along as one more group of the same two launches (its rows
         after the pairs'); with more it goes through the library."""
+        if isinstance(self.w_gate_up, ops.Fp8Weight):
+            return self._8_bits(x, ids, wts, ctx)
         T = x.shape[0]
         trace = ctx.extras.get("router_trace")
         if trace is not None:      # the picks of this step, layer by layer (reference: ForwardPass.cs:2042-2056)
@@ -365,6 +415,10 @@ class MoESwiGLU(Part):
             with section("router", nbytes=2 * T * self.hidden + 2 * self.E * self.hidden):
                 ids, wts = ops.router_topk(x, self.w_router, self.k, self.gate, self.renormalise, **self._route_args())
             return self._picked(x, ids, wts, ctx)
+        if isinstance(self.w_gate_up, ops.Fp8Weight):
+            with section("router", nbytes=2 * T * self.hidden + 2 * self.E * self.hidden):
+                ids, wts = ops.router_topk(x, self.w_router, self.k, self.gate, self.renormalise, **self._route_args())
+            return self._8_bits(x, ids, wts, ctx)
         many = self.MERGE_MIN_MANY_TOKENS is not None and T >= self.MERGE_MIN_MANY_TOKENS
         merge = self.merged and not self.identity and ctx.act_dtype == torch.bfloat16 and (T <= self.MERGE_MAX_TOKENS or many)
         with section("router", nbytes=2 * T * self.hidden + 2 * self.E * self.hidden):

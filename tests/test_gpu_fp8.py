@@ -265,3 +265,168 @@ def test_nothing_to_do():
     assert ops.feed_forward_fp8(x, p1.select(0), p2.select(0)).shape == (0, 96)
     ids, wts = torch.empty(0, 2, dtype=torch.int32, device=DEV), torch.empty(0, 2, device=DEV)
     assert ops.experts_fp8(x, ids, wts, p1, p2).shape == (0, 96)
+
+
+def _operators(g):
+    """name -> (inputs that change, call on them) of every operator, for few and many rows."""
+    from sharpinference_amd import ops
+    _, lin = _weight(g, 200, 384)
+    w1, w2, p1, p2 = _layer(g, 8, 384, 160, 200, True)
+    out = {}
+    for M in (1, 3, 16, 40, 130):
+        x = _normal(g, M, 384).bfloat16()
+        ids, wts = _picks(g, M, 8, 2)
+        out[f"rows {M}"] = ([x], lambda x: ops.quantize_rows(x).values())
+        out[f"gated rows {M}"] = ([_normal(g, M, 768)], lambda x: ops.quantize_rows(x, ops.ACT_SILU).values())
+        out[f"linear {M}"] = ([x], lambda x: ops.linear_fp8(x, lin))
+        out[f"feed forward {M}"] = ([x], lambda x: ops.feed_forward_fp8(x, p1.select(8), p2.select(8)))
+        out[f"experts {M}"] = ([x, ids, wts], lambda x, ids, wts: ops.experts_fp8(x, ids, wts, p1, p2, shared=True))
+    return out
+
+
+def test_captured_calls_replay_on_new_inputs():
+    g = _gen(5)
+    for name, (inputs, call) in _operators(g).items():
+        static = [t.clone() for t in inputs]
+        call(*static)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(*static)
+        for turn in range(4):
+            for s, t in zip(static, inputs):
+                s.copy_(t.flip(0) if turn % 2 else t)
+            want = call(*[t.clone() for t in static])          # (eager work between the replays)
+            torch.cuda.synchronize()
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want), (name, turn)
+
+
+def test_two_captured_layers_replayed_side_by_side():
+    """Graphs of one operator on two streams share nothing."""
+    g = _gen(6)
+    (inputs, call), graphs = _operators(g)["experts 3"], []
+    want = call(*inputs)
+    for _ in range(2):
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = call(*inputs)
+        graphs.append((stream, graph, out))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for stream, graph, _ in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for _, _, out in graphs)
+
+
+def test_calls_on_streams_of_their_own():
+    g = _gen(7)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for name, (inputs, call) in _operators(g).items():
+        want, got = call(*inputs), []
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for s in streams:
+                with torch.cuda.stream(s):
+                    got.append(call(*inputs))
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in got), name
+
+
+def test_a_run_of_them_as_a_layer_uses_them():
+    """Quantised once, multiplied twice: a projection and a layer of experts over the same rows, then the projection of their sum."""
+    from sharpinference_amd import ops
+    g = _gen(8)
+    _, lin = _weight(g, 384, 384)
+    _, _, p1, p2 = _layer(g, 4, 384, 160, 384, True)
+    for M in (2, 50, 300):
+        x = _normal(g, M, 384).bfloat16()
+        ids, wts = _picks(g, M, 4, 2)
+        q = ops.quantize_rows(x)
+        a, b = ops.linear_fp8(q, lin), ops.experts_fp8(q, ids, wts, p1, p2, shared=True)
+        assert torch.equal(a, ops.linear_fp8(x, lin)) and torch.equal(b, ops.experts_fp8(x, ids, wts, p1, p2, shared=True))
+        y = ops.linear_fp8(a + b, lin)
+        s, w = plain.rows(a + b), lin.values().double()
+        want = s @ w.T
+        assert ((y.double() - want).abs() <= plain.cut(s, w) + plain.stored(want)).all()
+
+
+def test_columns_behind_the_last_and_rows_beside_stay_as_they_are():
+    """A result's neighbours in memory are not written (odd sizes: stores of whole runs would pass the end)."""
+    from sharpinference_amd import ops
+    from sharpinference_amd.ops import fp8
+    g = _gen(9)
+    for M in (1, 5, 16, 33, 70, 200):
+        for N in (1, 33, 100, 257):
+            _, w = _weight(g, N, 256)
+            x = _normal(g, M, 256).bfloat16()
+            want = ops.linear_fp8(x, w)
+            q = ops.quantize_rows(x)
+            room = torch.full((M * N + 256,), 7.0, dtype=torch.bfloat16, device=DEV)
+            out = room[64:64 + M * N]
+            if M <= 64:
+                ops._run("sharpi_fp8_few", q.codes.data_ptr(), q.scales.data_ptr(), 2, w.codes.data_ptr(), w.scales.data_ptr(), w.stored_rows, out.data_ptr(),
+                         M, N, 256, 1, ops._stream())
+            else:
+                ops._run("sharpi_fp8_tiles", q.codes.data_ptr(), q.scales.data_ptr(), M, w.codes.data_ptr(), w.scales.data_ptr(), w.stored_rows,
+                         out.data_ptr(), 1, M, N, 256, None, None, 1, 0, 128, 2, 1, ops._stream())
+            torch.cuda.synchronize()
+            assert torch.equal(out.view(M, N), want) or ((out.view(M, N).double() - want.double()).abs() <= 2 * plain.stored(want.double()) + 1e-3).all()
+            assert (room[:64] == 7).all() and (room[64 + M * N:] == 7).all()
+    assert fp8.FP8_FEW_ROWS == 64
+
+
+@pytest.mark.parametrize("M,N,K", [(100, 96, 1100), (70, 513, 2048), (300, 100, 520)])
+@pytest.mark.parametrize("tile", [(64, 2, 1), (64, 2, 3), (128, 2, 2), (192, 1, 1), (192, 1, 4), (192, 2, 2), (256, 1, 3), (256, 2, 1), (256, 2, 4)])
+def test_products_in_every_kind_of_tile(monkeypatch, M, N, K, tile):
+    """Every height, width and number of shares, whatever the rule would choose."""
+    from sharpinference_amd import ops
+    from sharpinference_amd.ops import fp8
+    g = _gen(M, N, K)
+    x = (_normal(g, M, K) * torch.exp(_normal(g, M, 1))).bfloat16()
+    w, p = _weight(g, N, K)
+    monkeypatch.setattr(fp8, "tile_fp8", lambda *a: tile)
+    y = ops.linear_fp8(x, p)
+    a, b = plain.rows(x), plain.rows(w)
+    want = a @ b.T
+    assert ((y.double() - want).abs() <= plain.cut(a, b) + plain.stored(want)).all()
+
+
+@pytest.mark.parametrize("height", [64, 128, 192, 256])
+@pytest.mark.parametrize("T,E,k,shared", [(90, 4, 2, True), (700, 3, 1, False), (500, 2, 2, True)])
+def test_layers_in_every_height_of_tile(monkeypatch, T, E, k, shared, height):
+    from sharpinference_amd import ops
+    from sharpinference_amd.ops import fp8
+    g = _gen(T, E, k)
+    x = _whole(g, T, 256).bfloat16()
+    w1, w2, p1, p2 = _layer(g, E, 256, 200, 140, shared)
+    ids, wts = _picks(g, T, E, k)
+    monkeypatch.setattr(fp8, "grouped_tile_fp8", lambda *a: height)
+    y = ops.experts_fp8(x, ids, wts, p1, p2, shared=shared)
+    want, bound = _layer_want(x, ids, wts, w1, w2, "silu", False, shared)
+    assert ((y.double() - want).abs() <= bound + 2 ** -20 * want.abs() + plain.stored(want)).all()
+
+
+def test_refused_on_the_gpu():
+    from sharpinference_amd import ops
+    g = _gen(3)
+    _, w = _weight(g, 64, 128)
+    x = _normal(g, 4, 256).bfloat16()
+    for bad in (x, x[:, ::2], x[:, :128].half(), x[0, :128], ops.quantize_rows(x)):
+        with pytest.raises(ops.KernelError):
+            ops.linear_fp8(bad, w)
+    _, _, p1, p2 = _layer(g, 3, 128, 64, 96, False)
+    x, (ids, wts) = _normal(g, 4, 128).bfloat16(), _picks(g, 4, 3, 2)
+    for a, b in ((ids.long(), wts), (ids, wts.double()), (ids[:3], wts[:3]), (ids, wts[:, :1]), (ids.cpu(), wts), (ids.t().contiguous().t(), wts)):
+        with pytest.raises(ops.KernelError):
+            ops.experts_fp8(x, a, b, p1, p2)
+    with pytest.raises(ops.KernelError, match="not known"):
+        ops.experts_fp8(x, ids, wts, p1, p2, act=9)
+    with pytest.raises(ops.KernelError):
+        ops.feed_forward_fp8(x, p1.select(0), p2.select(0), act=(ops.ACT_SWISH_CLAMP, -1.0))
+    with pytest.raises(ops.KernelError):
+        ops.quantize_rows(_normal(g, 3, 5), ops.ACT_SILU)
