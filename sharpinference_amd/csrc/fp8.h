@@ -24,18 +24,16 @@ typedef __attribute__((ext_vector_type(8))) int i32x8;
 typedef __attribute__((ext_vector_type(4))) int i32x4;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
-typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
 
 constexpr int kF8Block = 128;                 // values that share a scale
 constexpr int kF8Tile = 32;                   // weight rows of a tile
 constexpr int kF8TileBytes = kF8Tile * kF8Block;
 constexpr uint32_t kF8Nan = 0x7f;
+constexpr int kF8MostK = 1 << 24;             // columns of a row at most: 256 rows of codes are 2^32 bytes, what a tile's loads reach
 
 static inline __host__ __device__ int f8_blocks(int k) { return (k + kF8Block - 1) / kF8Block; }
 static inline __host__ __device__ int f8_scale_stride(int k) { return (f8_blocks(k) + 3) & ~3; }     // bytes of a row's scales
 static inline __host__ __device__ int f8_padded_rows(int n) { return (n + kF8Tile - 1) / kF8Tile * kF8Tile; }
-// bytes of a stored matrix's scales (codes: padded rows x blocks x 128)
-static inline __host__ __device__ size_t f8_scale_bytes(int padded_rows, int k) { return (size_t)padded_rows * f8_scale_stride(k); }
 
 // The block's byte from the bits of its largest finite magnitude (448 = 1.75 x 2^8).
 __device__ __forceinline__ int f8_scale_of(uint32_t top_bits) {
@@ -45,7 +43,6 @@ __device__ __forceinline__ int f8_scale_of(uint32_t top_bits) {
 __device__ __forceinline__ float f8_scale_value(int s) { return __uint_as_float((uint32_t)s << 23); }
 
 typedef __attribute__((ext_vector_type(2))) short s16x2_t;
-typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2v_t;
 // Four values' codes, of floats or of two pairs of bfloat16, divided by `scale` (a power of two).
 __device__ __forceinline__ uint32_t f8_codes4(float a, float b, float c, float d, float scale) {

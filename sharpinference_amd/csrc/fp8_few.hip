@@ -4,10 +4,11 @@
 //   gated   h = act(s g) (s u) with (g | u) = q(x) W^T, rounded to bfloat16: the first half of a feed-forward, for one matrix or for the
 //           experts that a router picked (a block finds the rows of its expert among the picks itself)
 //   sum     out[t] = sum_j w[t, j] q(h[t, j]) W_e^T over the token's picks e (and an always-on expert): the second half, with the sum
-// q(.): up to 16 rows of bfloat16 are quantised by every block that reads them, into LDS (no launch and no pass of their own; the weights' first loads are on
+// q(.): a few rows of bfloat16 are quantised by every block that reads them, into LDS (no launch and no pass of their own; the weights' first loads are on
 // their way meanwhile); other rows come as codes.
 //
-// Bound: bytes of the weights.  Each wave takes blocks of 128 of k in turn, one 4 KB unit of a tile of 32 weight rows (or half of it)
+// Bound: bytes of the weights (13 rows of 202,048 x 5,120: 167 us, 6.3 TB/s; an expert of 8,192 x 5,120 and one always on, one token: 252 MB in 50 us with
+// both launches).  Each wave takes blocks of 128 of k in turn, one 4 KB unit of a tile of 32 weight rows (or half of it)
 // at a time through v_mfma_scale_f32_16x16x128: W is the A operand (rows = n), x the B operand (up to 16 rows a row block).  A lane ends
 // up with four neighbouring n of one x row; the waves' sums meet in LDS and are added in wave order.
 //
@@ -23,6 +24,8 @@ constexpr int FW = 8;                  // waves a block
 constexpr int kFewRows = 64;           // rows (tokens) of a call at most: four row blocks
 constexpr int kFewPairs = 512;         // (token, pick) pairs of a call at most
 constexpr int kFewExperts = 1024;
+constexpr int kStagedRows = 2;         // rows of bfloat16 that the kernels quantise themselves
+constexpr int kLayerTiles = 2;         // half tiles a block of a layer's two products
 constexpr int kRound = 2;              // (tile, row block) pairs that meet in LDS at a time
 
 struct F8Matrix {
@@ -39,20 +42,21 @@ struct F8Picks {
   int shared;              // one more matrix (number E) that every token goes through: rows T k + t
 };
 
-// A wave's view of one 16-row half tile of a matrix.
+// A wave's view of one 16-row half tile of a matrix: addresses that the wave shares, and a lane's 32-bit offsets from them.
 struct F8Lane {
   const uint8_t* codes;
   const uint8_t* scales;
-  __device__ __forceinline__ void at(const F8Matrix& w, size_t matrix, int half_tile, int r, int g) {
+  __device__ __forceinline__ void at(const F8Matrix& w, size_t matrix, int half_tile) {
     const int last = w.rows / 16 - 1, t = half_tile < last ? half_tile : last;      // (beyond the last: read, never stored)
     const size_t tile = matrix * (w.rows / 32) + (t >> 1);
-    codes = w.codes + tile * w.U * kF8TileBytes + (g >> 1) * 2048 + (g & 1) * 512 + (t & 1) * 256 + r * 16;
-    scales = w.scales + tile * ((w.U + 3) >> 2) * 128 + ((t & 1) * 16 + r) * 4;
+    codes = w.codes + tile * w.U * kF8TileBytes + (t & 1) * 256;
+    scales = w.scales + tile * ((w.U + 3) >> 2) * 128 + (t & 1) * 64;
   }
-  __device__ __forceinline__ i32x8 load(int u, int& s) const {
-    const i32x4 a = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(codes + (size_t)u * kF8TileBytes));
-    const i32x4 b = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(codes + (size_t)u * kF8TileBytes + 1024));
-    s = scales[(u >> 2) * 128 + (u & 3)];
+  __device__ __forceinline__ i32x8 load(int u, int r, int g, int& s) const {
+    const uint8_t* from = codes + (size_t)u * kF8TileBytes + (uint32_t)((g >> 1) * 2048 + (g & 1) * 512 + r * 16);
+    const i32x4 a = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(from));
+    const i32x4 b = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(from + 1024));
+    s = (scales + (u >> 2) * 128 + (u & 3))[(uint32_t)r * 4];
     return i32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   }
 };
@@ -119,11 +123,12 @@ template <typename F> __device__ __forceinline__ void stage_rows(const bf16_t* _
 struct F8Row {
   i32x4 a, b;
   int byte;
-  __device__ __forceinline__ void load(const void* x, const uint8_t* scales, size_t row, int K, int u, int g) {
-    const uint8_t* p = (const uint8_t*)x + (row * f8_blocks(K) + u) * kF8Block + g * 32;
+  // OFFSET: of the row's lane piece and of its bytes, 32 bits where the rows lie within 4 GB
+  template <typename OFFSET> __device__ __forceinline__ void load(const void* x, const uint8_t* scales, OFFSET at, OFFSET scale_at, int u) {
+    const uint8_t* p = (const uint8_t*)x + (size_t)u * kF8Block + at;
     a = *reinterpret_cast<const i32x4*>(p);
     b = *reinterpret_cast<const i32x4*>(p + 16);
-    byte = scales[row * f8_scale_stride(K) + u];
+    byte = (scales + u)[scale_at];
   }
   __device__ __forceinline__ i32x8 codes(int& s) const {
     s = byte;
@@ -176,11 +181,11 @@ __device__ __forceinline__ void store_columns(bf16_t* row, int n, int columns, c
 
 // plain and gated.  R half tiles a block: of distinct columns (plain), or R / 2 of gate columns and the up columns beside them (gated).
 // n_out: columns of the result that exist; stride: of a stored row (gated: the columns from n_out to it are zeros, as their weights are).
-// STAGED: x is bfloat16, up to 16 rows, quantised into LDS (turn: rows that fit there at a time); else codes.  A block of the plain form takes every gridDim.x-th column group.
+// STAGED: x is bfloat16, up to kStagedRows rows, quantised into LDS, `turn` of an expert's at a time; else codes.
 template <int R, int MB, bool STAGED, bool GATED>
 __global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_few_kernel(const void* __restrict__ x, const uint8_t* __restrict__ x_scales, F8Matrix W,
                                                                             bf16_t* __restrict__ out, int n_out, int stride, int M, int K, GatedAct act,
-                                                                            F8Picks pk, int* __restrict__ clear, int n_clear, int turn, int column_groups) {
+                                                                            F8Picks pk, int* __restrict__ clear, int n_clear, int turn) {
   static_assert(!STAGED || MB == 1, "staged rows are one row block");
   extern __shared__ __attribute__((aligned(16))) uint8_t staged_bytes[];
   constexpr int TG = GATED ? R / 2 : R;
@@ -232,6 +237,7 @@ __global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_few_kernel(cons
           before += n;
         }
       }
+      expert = __builtin_amdgcn_readfirstlane(expert);
       if (expert < 0) return;                   // (the same for the block)
       if (w == 0) {
         int n = 0;
@@ -244,7 +250,7 @@ __global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_few_kernel(cons
         if (lane == 0) n_members = n;
       }
       __syncthreads();
-      rows = n_members;
+      rows = __builtin_amdgcn_readfirstlane(n_members);
     }
   }
   if (rows <= 0) return;
@@ -255,17 +261,20 @@ __global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_few_kernel(cons
   for (int rb = 0; rb < rows; rb += group_rows) {
     const int here = min(rows - rb, group_rows);            // rows of this turn
     const F8Staged st{staged_bytes, staged_bytes + W.U * kF8Block * here, here};
-    size_t xr[MB];
+    // (staged: the row; codes: offsets, of up to 64 rows)
+    uint32_t xr[MB], xsr[MB];
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb) xr[mb] = STAGED ? min(r, here - 1) : x_row(rb + min(mb * 16 + r, here - 1));
-    bool fresh = STAGED;                                    // (the rows are still to be staged)
-    for (int cg = blockIdx.x; cg < column_groups; cg += gridDim.x) {
-    const int n_base = cg * 16 * TG;
+    for (int mb = 0; mb < MB; ++mb) {
+      const uint32_t row = STAGED ? min(r, here - 1) : x_row(rb + min(mb * 16 + r, here - 1));
+      xr[mb] = STAGED ? row : row * (W.U * kF8Block) + g * 32;
+      xsr[mb] = row * f8_scale_stride(K);
+    }
+    const int n_base = blockIdx.x * 16 * TG;
     F8Lane wl[R];
     // (of a gated matrix the up rows begin at half its rows, a multiple of 32: half tile rows / 32)
 #pragma unroll
     for (int t = 0; t < R; ++t)
-      wl[t].at(W, expert, n_base / 16 + t % TG + (GATED && t >= TG ? W.rows / 32 : 0), r, g);
+      wl[t].at(W, expert, n_base / 16 + t % TG + (GATED && t >= TG ? W.rows / 32 : 0));
     f32x4 acc[R][MB];
 #pragma unroll
     for (int t = 0; t < R; ++t)
@@ -278,10 +287,10 @@ __global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_few_kernel(cons
     };
     auto load_unit = [&](int u, Unit& un) {
 #pragma unroll
-      for (int t = 0; t < R; ++t) un.wf[t] = wl[t].load(u, un.ws[t]);
+      for (int t = 0; t < R; ++t) un.wf[t] = wl[t].load(u, r, g, un.ws[t]);
       if constexpr (!STAGED) {
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb) un.xf[mb].load(x, x_scales, xr[mb], K, u, g);     // (a row block without rows reads the last row)
+        for (int mb = 0; mb < MB; ++mb) un.xf[mb].load(x, x_scales, xr[mb], xsr[mb], u);     // (a row block without rows reads the last row)
       }
     };
     auto use_unit = [&](int u, Unit& un) {
@@ -301,16 +310,13 @@ __global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_few_kernel(cons
     int u = w;
     if (u < W.U) load_unit(u, a);
     if constexpr (STAGED) {
-      if (fresh) {
-        if (rb > 0) __syncthreads();                        // (the turn before has been read)
-        stage_rows((const bf16_t*)x, K, here * W.U, st, [&](int task, int& row, int& block, int& to, int& m) {
-          m = task / W.U;
-          block = to = task - m * W.U;
-          row = x_row(rb + m);
-        });
-        __syncthreads();
-        fresh = false;
-      }
+      if (rb > 0) __syncthreads();                          // (the turn before has been read)
+      stage_rows((const bf16_t*)x, K, here * W.U, st, [&](int task, int& row, int& block, int& to, int& m) {
+        m = task / W.U;
+        block = to = task - m * W.U;
+        row = x_row(rb + m);
+      });
+      __syncthreads();
     }
     for (; u + 2 * FW < W.U; u += 2 * FW) {
       load_unit(u + FW, b);
@@ -375,13 +381,12 @@ __global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_few_kernel(cons
         }
       }
     }
-    }
   }
 }
 
 // The sum over a token's picks.  R half tiles of columns a block, MB row blocks of tokens; blockIdx.y: the share of the blocks of k.
 // part [S][tiles][MB][R][64 lanes] float4, counters [tiles] zero before the launch (both unused if S is 1).
-// STAGED: h is bfloat16, up to 16 tokens, quantised into LDS `chunk` blocks of k (a multiple of 2 FW) at a time; else codes.
+// STAGED: h is bfloat16, up to kStagedRows tokens, quantised into LDS `chunk` blocks of k (a multiple of 2 FW) at a time; else codes.
 template <int R, int MB, bool STAGED>
 __global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_sum_kernel(const void* __restrict__ h, const uint8_t* __restrict__ h_scales, F8Matrix W,
                                                                             bf16_t* __restrict__ out, int n_out, int K, F8Picks pk, int weighted,
@@ -431,7 +436,7 @@ __global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_sum_kernel(cons
     __syncthreads();
   }
   const int entries = pk.ids ? __builtin_amdgcn_readfirstlane(n_entries) : 1;
-  const int S = gridDim.y, share = blockIdx.y, all = entries * W.U;      // (entries x blocks of k: below 2^31, checked on the host)
+  const int S = gridDim.y, share = blockIdx.y, all = entries * W.U;      // (entries x blocks of k: up to 513 x 2^17)
   const int first = (int)((long long)all * share / S), end = (int)((long long)all * (share + 1) / S);
   const int n_base = blockIdx.x * 16 * R;
 
@@ -474,13 +479,14 @@ __global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_sum_kernel(cons
 #pragma unroll
     for (int t = 0; t < R; ++t) {
       F8Lane wl;
-      wl.at(W, code & 0xffff, n_base / 16 + t, r, g);
-      un.wf[t] = wl.load(u, un.ws[t]);
+      wl.at(W, code & 0xffff, n_base / 16 + t);
+      un.wf[t] = wl.load(u, r, g, un.ws[t]);
     }
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
       un.row[mb] = row_of(code, mb * 16 + r, un.weight[mb]);
-      if constexpr (!STAGED) un.xf[mb].load(h, h_scales, max(un.row[mb], 0), K, u, g);      // (row 0: read for a token without this expert, never added)
+      const size_t row = max(un.row[mb], 0);
+      if constexpr (!STAGED) un.xf[mb].load(h, h_scales, row * (W.U * kF8Block) + g * 32, row * f8_scale_stride(K), u);      // (row 0: read for a token without this expert, never added)
     }
   };
   const F8Staged st{staged_bytes, staged_bytes + chunk * kF8Block * pk.T, pk.T};
@@ -570,16 +576,17 @@ __global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_sum_kernel(cons
   }
 }
 
-// x operand of a call: codes, or (up to 16 rows) bfloat16 whose runs of eight lie at 16-byte addresses
+// x operand of a call: codes, or (up to kStagedRows rows) bfloat16 whose runs of eight lie at 16-byte addresses
 enum : int { X_BF16 = DT_BF16, X_CODES = 2 };
 constexpr int kStagedMost = 48 * 1024;          // bytes of LDS for staged rows
+constexpr int kMostAcross = 0x7fffff;           // blocks of a launch along x (of 512 threads each, of which there are at most 2^32)
 bool rows_ok(const void* x, int kind, int M, int K) {
   if (((uintptr_t)x & 15) != 0) return false;
-  return kind == X_CODES || (kind == X_BF16 && K % 8 == 0 && M <= 16);
+  return kind == X_CODES || (kind == X_BF16 && K % 8 == 0 && M <= kStagedRows);
 }
 int staged_size(int rows, int blocks) { return rows * blocks * (kF8Block + 1) + 16; }
 bool matrix_ok(const F8Matrix& W, long long matrices) {
-  return W.rows > 0 && W.rows % kF8Tile == 0 && W.U > 0 && matrices > 0 && (long long)W.rows * W.U < 0x7fffffffLL;
+  return W.rows > 0 && W.rows % kF8Tile == 0 && W.U > 0 && matrices > 0 && (long long)W.rows * W.U < 0x7fffffffLL && !(((uintptr_t)W.codes) & 15);
 }
 
 }  // namespace
@@ -589,23 +596,20 @@ SHARPI_EXPORT int sharpi_fp8_few(const void* x, const void* x_scales, int kind, 
                                  int M, int N, int K, int R, hipStream_t stream) {
   if (M <= 0) return SHARPI_OK;
   const F8Matrix W{(const uint8_t*)w_codes, (const uint8_t*)w_scales, w_rows, f8_blocks(K)};
-  if (M > kFewRows || N <= 0 || K <= 0 || w_rows != f8_padded_rows(N) || !matrix_ok(W, 1) || !rows_ok(x, kind, M, K)) return SHARPI_ERR_ARG;
+  if ((R != 1 && R != 2) || M > kFewRows || N <= 0 || K <= 0 || K >= kF8MostK || w_rows != f8_padded_rows(N) || !matrix_ok(W, 1) || !rows_ok(x, kind, M, K)) return SHARPI_ERR_ARG;
   const int mb = M <= 16 ? 1 : M <= 32 ? 2 : 4, groups = ceil_div(N, 16 * R);
   const int lds = kind == X_CODES ? 0 : staged_size(M, W.U);
-  if (lds > kStagedMost) return SHARPI_ERR_ARG;
-  // (as many blocks as stay at once: each stages the rows for all its column groups)
-  const int most = lds ? 4 * compute_units() : groups;
-  const dim3 grid((unsigned)(groups < most ? groups : most)), block(FW * kWave);
+  if (lds > kStagedMost || groups > kMostAcross) return SHARPI_ERR_ARG;
+  const dim3 grid((unsigned)groups), block(FW * kWave);
 #define FF(RV, MBV, STG) \
-  fp8_few_kernel<RV, MBV, STG, false><<<grid, block, lds, stream>>>(x, (const uint8_t*)x_scales, W, (bf16_t*)out, N, N, M, K, GatedAct{}, F8Picks{}, nullptr, 0, M, groups)
+  fp8_few_kernel<RV, MBV, STG, false><<<grid, block, lds, stream>>>(x, (const uint8_t*)x_scales, W, (bf16_t*)out, N, N, M, K, GatedAct{}, F8Picks{}, nullptr, 0, M)
 #define FF_X(RV)                          \
   if (kind != X_CODES) FF(RV, 1, true);   \
   else if (mb == 1) FF(RV, 1, false);     \
   else if (mb == 2) FF(RV, 2, false);     \
   else FF(RV, 4, false)
   if (R == 1) { FF_X(1); }
-  else if (R == 2) { FF_X(2); }
-  else return SHARPI_ERR_ARG;
+  else { FF_X(2); }
 #undef FF_X
 #undef FF
   SHARPI_CHECK_LAUNCH();
@@ -623,59 +627,50 @@ static bool picks_ok(const F8Picks& p) {
 // clear [n_clear]: set to zero (the counters of the launch behind).
 SHARPI_EXPORT int sharpi_fp8_few_gated(const void* x, const void* x_scales, int kind, const void* w_codes, const void* w_scales, int w_rows, void* h,
                                        int stride, const int* ids, const float* wts, int T, int k, int E, int shared, int I, int K, int act, float limit,
-                                       int R, int* clear, int n_clear, hipStream_t stream) {
+                                       int* clear, int n_clear, hipStream_t stream) {
   if (T <= 0) return SHARPI_OK;
   const F8Matrix W{(const uint8_t*)w_codes, (const uint8_t*)w_scales, w_rows, f8_blocks(K)};
   const F8Picks pk{ids, wts, T, k, E, shared ? 1 : 0};
   const GatedAct ga{act, limit};
-  if (I <= 0 || K <= 0 || w_rows != 2 * f8_padded_rows(I) || stride != (I + 7) / 8 * 8 || !act_known(ga) || !picks_ok(pk) ||
+  if (I <= 0 || K <= 0 || K >= kF8MostK || w_rows != 2 * f8_padded_rows(I) || stride != (I + 7) / 8 * 8 || !act_known(ga) || !picks_ok(pk) ||
       !matrix_ok(W, E + pk.shared) || !rows_ok(x, kind, T, K) || ((uintptr_t)h & 15)) return SHARPI_ERR_ARG;
   const int mb = T <= 16 ? 1 : T <= 32 ? 2 : 4;
-  const int groups = ids ? (T * k < E ? T * k : E) + pk.shared : 1, column_groups = ceil_div(I, 8 * R);
+  const int groups = ids ? (T * k < E ? T * k : E) + pk.shared : 1, column_groups = ceil_div(I, 8 * kLayerTiles);
   const int lds = kind == X_CODES ? 0 : staged_size(T, W.U);       // (rows of a turn: the tokens')
-  if (lds > kStagedMost) return SHARPI_ERR_ARG;
+  if (lds > kStagedMost || column_groups > kMostAcross) return SHARPI_ERR_ARG;
   const dim3 grid((unsigned)column_groups, (unsigned)groups), block(FW * kWave);
-#define FG(RV, MBV, STG) \
-  fp8_few_kernel<RV, MBV, STG, true><<<grid, block, lds, stream>>>(x, (const uint8_t*)x_scales, W, (bf16_t*)h, I, stride, T, K, ga, pk, clear, n_clear, T, column_groups)
-#define FG_X(RV)                          \
-  if (kind != X_CODES) FG(RV, 1, true);   \
-  else if (mb == 1) FG(RV, 1, false);     \
-  else if (mb == 2) FG(RV, 2, false);     \
-  else FG(RV, 4, false)
-  if (R == 2) { FG_X(2); }
-  else return SHARPI_ERR_ARG;
-#undef FG_X
+#define FG(MBV, STG) \
+  fp8_few_kernel<kLayerTiles, MBV, STG, true><<<grid, block, lds, stream>>>(x, (const uint8_t*)x_scales, W, (bf16_t*)h, I, stride, T, K, ga, pk, clear, n_clear, T)
+  if (kind != X_CODES) FG(1, true);
+  else if (mb == 1) FG(1, false);
+  else if (mb == 2) FG(2, false);
+  else FG(4, false);
 #undef FG
   SHARPI_CHECK_LAUNCH();
   return SHARPI_OK;
 }
 
 // out [T, N] bfloat16 = the sum over the picks of q(h row) W_e^T (times the pair's weight if wts is given), plus the always-on expert's.
-// h [T k (+ T), K]: bfloat16 (T <= 16, K a multiple of 8) or codes.  S shares of the blocks of k; part: S x tiles x 1 KB x R x row blocks; counters [tiles] zero.
+// h [T k (+ T), K]: bfloat16 (up to kStagedRows tokens, K a multiple of 8) or codes.  S shares of the blocks of k for each tile of 16 kLayerTiles columns; part: S x
+// tiles x 1 KB x kLayerTiles x row blocks; counters [tiles] zero.
 SHARPI_EXPORT int sharpi_fp8_few_sum(const void* h, const void* h_scales, int kind, const void* w_codes, const void* w_scales, int w_rows, void* out, const int* ids, const float* wts,
-                                     int T, int k, int E, int shared, int N, int K, int R, int S, void* part, int* counters, hipStream_t stream) {
+                                     int T, int k, int E, int shared, int N, int K, int S, void* part, int* counters, hipStream_t stream) {
   if (T <= 0) return SHARPI_OK;
   const F8Matrix W{(const uint8_t*)w_codes, (const uint8_t*)w_scales, w_rows, f8_blocks(K)};
   const F8Picks pk{ids, wts, T, k, E, shared ? 1 : 0};
-  if (N <= 0 || K <= 0 || w_rows != f8_padded_rows(N) || !picks_ok(pk) || !matrix_ok(W, E + pk.shared) || !rows_ok(h, kind, T, K) || S < 1 ||
-      (S > 1 && (!part || !counters)) || (long long)(kFewPairs + 1) * W.U > 0x7fffffffLL) return SHARPI_ERR_ARG;
+  if (N <= 0 || K <= 0 || K >= kF8MostK || w_rows != f8_padded_rows(N) || !picks_ok(pk) || !matrix_ok(W, E + pk.shared) || !rows_ok(h, kind, T, K) || S < 1 ||
+      S > 0xffff || (S > 1 && (!part || !counters)) || ceil_div(N, 16 * kLayerTiles) > kMostAcross) return SHARPI_ERR_ARG;
   const int mb = T <= 16 ? 1 : T <= 32 ? 2 : 4;
-  const dim3 grid((unsigned)ceil_div(N, 16 * R), (unsigned)S), block(FW * kWave);
-  // blocks of k staged at a time: up to 32 KB of rows
-  const int chunk = T <= 8 ? 4 * FW : 2 * FW;
+  const dim3 grid((unsigned)ceil_div(N, 16 * kLayerTiles), (unsigned)S), block(FW * kWave);
+  constexpr int chunk = 4 * FW;                       // blocks of k staged at a time: up to 16 KB of rows
   const int lds = kind == X_CODES ? 0 : staged_size(T, chunk);
-#define FS(RV, MBV, STG) \
-  fp8_sum_kernel<RV, MBV, STG><<<grid, block, lds, stream>>>(h, (const uint8_t*)h_scales, W, (bf16_t*)out, N, K, pk, wts != nullptr, (f32x4*)part, counters, \
+#define FS(MBV, STG) \
+  fp8_sum_kernel<kLayerTiles, MBV, STG><<<grid, block, lds, stream>>>(h, (const uint8_t*)h_scales, W, (bf16_t*)out, N, K, pk, wts != nullptr, (f32x4*)part, counters, \
                                                              STG ? chunk : 0x40000000)
-#define FS_MB(RV)                       \
-  if (kind != X_CODES) FS(RV, 1, true); \
-  else if (mb == 1) FS(RV, 1, false);   \
-  else if (mb == 2) FS(RV, 2, false);   \
-  else FS(RV, 4, false)
-  if (R == 1) { FS_MB(1); }
-  else if (R == 2) { FS_MB(2); }
-  else return SHARPI_ERR_ARG;
-#undef FS_MB
+  if (kind != X_CODES) FS(1, true);
+  else if (mb == 1) FS(1, false);
+  else if (mb == 2) FS(2, false);
+  else FS(4, false);
 #undef FS
   SHARPI_CHECK_LAUNCH();
   return SHARPI_OK;

@@ -434,9 +434,10 @@ __global__ __launch_bounds__(TW* kWave, PAIRED ? 4 : 2) void fp8_tiles_kernel(F8
 }
 
 bool tiles_ok(const F8Tiles& p, int x_rows) {
-  return p.rows > 0 && x_rows > 0 && p.U > 0 && p.w_rows > 0 && p.w_rows % kF8Tile == 0 && p.groups > 0 && p.groups < kMaxGroups && p.along >= 0 && (p.offsets || !p.along) && (long long)p.rows + p.along <= 0x7fffffffLL &&
-         (long long)p.w_rows * p.U < 0x7fffffffLL && !(((uintptr_t)p.x | (uintptr_t)p.w) & 15) && (p.offsets || p.groups == 1) &&
-         (!p.a_rows || (long long)x_rows * p.U * kF8Block <= 0xffffffffLL) && (long long)p.U * kF8TileBytes <= 0x7fffffffLL;
+  return p.rows > 0 && x_rows > 0 && p.U > 0 && p.U <= f8_blocks(kF8MostK - 1) && p.w_rows > 0 && p.w_rows % kF8Tile == 0 && p.groups > 0 && p.groups < kMaxGroups &&
+         p.along >= 0 && (p.offsets || !p.along) && (long long)p.rows + p.along <= 0x7fffff00LL && (long long)p.w_rows * p.U < 0x7fffffffLL &&
+         !(((uintptr_t)p.x | (uintptr_t)p.w) & 15) && !(((uintptr_t)p.xs | (uintptr_t)p.ws) & 3) && (p.offsets || p.groups == 1) &&
+         (!p.a_rows || (long long)x_rows * p.U * kF8Block <= 0xffffffffLL);
 }
 
 template <bool GATED> int launch_tiles(F8Tiles p, const F8Out& o, GatedAct act, int nt, int dtype, hipStream_t stream) {
@@ -447,7 +448,7 @@ template <bool GATED> int launch_tiles(F8Tiles p, const F8Out& o, GatedAct act, 
   if ((nt != 1 && nt != 2) || (nt == 1 && (GATED || height <= 64 * Ring<true>::kHighest))) return SHARPI_ERR_ARG;
   p.nb = ceil_div(o.n_out, GATED ? columns_of(nt) / 2 : columns_of(nt));
   p.tiles = (int)tiles;
-  if (tiles * p.nb > 0x7fffffffLL) return SHARPI_ERR_ARG;
+  if (tiles * p.nb > 0x7fffff) return SHARPI_ERR_ARG;        // (of 512 threads each, of which a launch has at most 2^32 along x)
   if (p.shares < 1 || p.shares > p.U || (p.shares > 1 && (GATED || p.offsets || dtype != DT_F32))) return SHARPI_ERR_ARG;
   const dim3 grid((unsigned)(tiles * p.nb), (unsigned)p.shares), block(TW * kWave);
   if constexpr (!GATED) {

@@ -656,7 +656,7 @@ __device__ void permute_block(const int* __restrict__ topk_ids, const float* __r
 #pragma unroll
     for (int x = 0; x < KEEP; ++x) {
       if (x % kAhead == 0 && x * step >= n_pairs) break;
-      const bool real = tid + x * step < n_pairs && pair[x] < n_experts;
+      const bool real = tid + x * step < n_pairs && (unsigned)pair[x] < (unsigned)n_experts;
       const int c = counter(pair[x]);
       const int was = atomicAdd(real ? counters + c : mine, 1);
       pair[x] = real ? was * kPermuteCounters + c : -1;
@@ -668,7 +668,7 @@ __device__ void permute_block(const int* __restrict__ topk_ids, const float* __r
       for (int x = 0; x < kAhead; ++x) id[x] = topk_ids[min(i0 + x * step, n_pairs - 1)];
 #pragma unroll
       for (int x = 0; x < kAhead; ++x)
-        if (i0 + x * step < n_pairs && id[x] < n_experts) atomicAdd(counters + counter(id[x]), 1);
+        if (i0 + x * step < n_pairs && (unsigned)id[x] < (unsigned)n_experts) atomicAdd(counters + counter(id[x]), 1);
     }
   }
   __syncthreads();
@@ -806,7 +806,7 @@ __device__ void permute_block(const int* __restrict__ topk_ids, const float* __r
       }
 #pragma unroll
       for (int x = 0; x < kAhead; ++x)
-        row[x] = i0 + x * step < n_pairs && id[x] < n_experts ? atomicAdd(counters + counter(id[x]), 1) : -1;
+        row[x] = i0 + x * step < n_pairs && (unsigned)id[x] < (unsigned)n_experts ? atomicAdd(counters + counter(id[x]), 1) : -1;
 #pragma unroll
       for (int x = 0; x < kAhead; ++x)
         if (const int i = i0 + x * step; i < n_pairs) {

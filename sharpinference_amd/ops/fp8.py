@@ -20,11 +20,18 @@ from . import ACT_SILU, _code, _dev, _i32, _known_act_pair, _need, _ptr, _run, c
 FP8_BLOCK = 128                # values that share a scale
 FP8_TILE = 32                  # weight rows of a stored tile
 FP8_FEW_ROWS = 64              # rows of the weight-streaming kernels (csrc/fp8_few.hip kFewRows)
-FP8_FEW_TOKENS = 16            # tokens of a layer that takes the picks as they are
+# tokens of a layer that takes the picks as they are (us, so and sorted by expert: one of 16 experts of 5,120 x 8,192 and one always on, 8 tokens 146 and 203, 16 222 and
+# 285, 17 272 and 271, 24 305 and 291; six of 64 of 2,048 x 1,408, 8 tokens 69 and 76, 16 90 and 88, 17 121 and 96)
+FP8_FEW_TOKENS = 16
 FP8_FEW_PAIRS = 512            # (token, pick) pairs of the same (kFewPairs)
+FP8_LAYER_COLUMNS = 32         # columns of the sum that a block takes (16 kLayerTiles)
 FP8_MAX_EXPERTS = 1023         # experts of a layer, one more may be always on (kFewExperts, kMaxGroups)
-FP8_STAGED_ROWS = 4
-FP8_STAGED_SUM = 2
+FP8_MOST_K = (1 << 24) - 1     # columns of a row (kF8MostK)
+# rows of bfloat16 that the weight-streaming kernels quantise where they read them, in every block, instead of in a launch ahead (us of a layer's launches, staged
+# and ahead: an expert of 16 of 5,120 x 8,192 and one always on, 1 token 54.6 and 55.8, 2 73.0 and 76.3, 4 108.7 and 103.6, 8 164 and 142; six of 64 of 2,048 x 1,408, 1 token
+# 26.0 and 28.1, 2 35.9 and 38.6, 4 51.7 and 49.5)
+FP8_STAGED_ROWS = 2
+FP8_STAGED_COLUMNS = 32768     # columns of a single product that does (5,120 x 7,168, 1 row 9.6 and 11.1; 5,120 x 202,048, 1 row 166 and 156)
 FP8_STAGED_BYTES = 48 * 1024   # LDS for rows that are quantised where they are read (kStagedMost)
 _F32, _BF16 = _code(torch.float32), _code(torch.bfloat16)
 _X_CODES = 2                   # csrc/fp8_few.hip X_CODES
@@ -121,6 +128,10 @@ class Fp8Weight:
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, gated: bool):
         self.codes, self.scales, self.shape, self.gated = codes, scales, tuple(shape), bool(gated)
+        lead, tiles, K = self.shape[:-2], self.stored_rows // FP8_TILE, self.shape[-1]
+        _need(codes.dtype == scales.dtype == torch.uint8 and codes.device == scales.device and codes.is_contiguous() and scales.is_contiguous()
+              and tuple(codes.shape) == (*lead, tiles, _blocks(K), FP8_TILE * FP8_BLOCK) and tuple(scales.shape) == (*lead, tiles, _scale_stride(K) // 4, FP8_TILE, 4),
+              f"Fp8Weight: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not those of {self.shape}")
 
     def dim(self) -> int:
         return len(self.shape)
@@ -168,6 +179,7 @@ def _new_weight(shape, gated: bool, device) -> Fp8Weight:
           f"8-bit weights must be [N, K] or [E, N, K] with at most {FP8_MAX_EXPERTS + 1} matrices")
     N, K = shape[-2:]
     _need(not gated or N % 2 == 0, "a gated matrix holds gate rows, then as many up rows")
+    _need(K <= FP8_MOST_K, f"8-bit rows have up to {FP8_MOST_K} columns")
     R = 2 * _padded(N // 2) if gated else _padded(N)
     _need(R * _blocks(K) <= 0x7fffffff, f"8-bit weights [{N}, {K}] are too large")
     lead = tuple(shape[:-2])
@@ -246,6 +258,7 @@ def quantize_rows(x: torch.Tensor, act=None) -> Fp8Rows:
     code, limit = (0, 0.0) if act is None else _known_act_pair(act)
     _need(not code or x.shape[1] % 2 == 0, "quantize_rows: a gated input is [M, 2I]")
     M, K = x.shape[0], x.shape[1] // (2 if code else 1)
+    _need(K <= FP8_MOST_K and M < 1 << 31, f"quantize_rows: up to {FP8_MOST_K} columns")
     out = _new_rows(M, K, x.device)
     with _device_of(x):
         _run("sharpi_fp8_rows", x.data_ptr(), dt, out.codes.data_ptr(), out.scales.data_ptr(), M, K, code, limit, _stream_of(x))
@@ -291,7 +304,8 @@ def _rows_checked(x, k: int, who: str) -> None:
 
 
 def linear_fp8(x: Union[torch.Tensor, Fp8Rows], w: Fp8Weight) -> torch.Tensor:
-    """x [M, K] W^T in 8 bits: bfloat16 [M, N].  A few rows go by streaming the weights, more in tiles (``few_rows_fp8``, ``tile_fp8``)."""
+    """x [M, K] W^T in 8 bits: bfloat16 [M, N].  A few rows go by streaming the weights (one or two of bfloat16 in a launch), more in tiles (``few_rows_fp8``,
+    ``tile_fp8``)."""
     _need(isinstance(w, Fp8Weight) and w.dim() == 2 and not w.gated, "linear_fp8: w must be an Fp8Weight [N, K], not gated")
     N, K = w.shape
     _rows_checked(x, K, "linear_fp8")
@@ -302,7 +316,7 @@ def linear_fp8(x: Union[torch.Tensor, Fp8Rows], w: Fp8Weight) -> torch.Tensor:
         return out
     few = few_rows_fp8(M, N)
     scratch = _Scratch()
-    rows = _Operand(x, scratch, few and _staged(x))
+    rows = _Operand(x, scratch, few and N <= FP8_STAGED_COLUMNS and _staged(x))
     product = None if few else _Tiled(M, N, K, scratch)
     if scratch.size:
         scratch.make(out.device)
@@ -403,14 +417,14 @@ def _few_layer(x, ids, wts, w1: Fp8Weight, w2: Fp8Weight, code: int, limit: floa
     k, also = 1 if ids is None else ids.shape[1], 1 if shared else 0
     rows, stride = T * k + also * T, -(-inner // 8) * 8
     met = min(E, T * k) + also if ids is not None else 1
-    tiles = -(-N // (16 * SUM_TILES))
+    tiles = -(-N // FP8_LAYER_COLUMNS)
     shares = sum_shares(tiles, met * _blocks(inner), compute_units())
     row_blocks = 1 if T <= 16 else 2 if T <= 32 else 4
     scratch = _Scratch()
     h, counters = scratch.add(rows * stride * 2), scratch.add(tiles * 4)
-    part = scratch.add(shares * tiles * SUM_TILES * row_blocks * 1024 if shares > 1 else 0)
+    part = scratch.add(shares * tiles * FP8_LAYER_COLUMNS * row_blocks * 64 if shares > 1 else 0)
     operand = _Operand(x, scratch, _staged(x))
-    if T > FP8_STAGED_SUM:
+    if T > FP8_STAGED_ROWS:
         codes, scales_at = scratch.add(rows * _blocks(stride) * FP8_BLOCK), scratch.add(rows * _scale_stride(stride))
     scratch.make(w1.codes.device)
     out = torch.empty((T, N), dtype=torch.bfloat16, device=w1.codes.device)
@@ -418,17 +432,14 @@ def _few_layer(x, ids, wts, w1: Fp8Weight, w2: Fp8Weight, code: int, limit: floa
     a, scales, kind = operand.ready(scratch, stream)
     w_in, w_out = (_ptr(wts), None) if on_input else (None, _ptr(wts))
     _run("sharpi_fp8_few_gated", a, scales, kind, w1.codes.data_ptr(), w1.scales.data_ptr(), w1.stored_rows, scratch[h], stride, ids_at, w_in,
-         T, k, E, also, inner, K, code, limit, 2, scratch[counters], tiles, stream)
+         T, k, E, also, inner, K, code, limit, scratch[counters], tiles, stream)
     a, scales, kind = scratch[h], None, _BF16
-    if T > FP8_STAGED_SUM:
+    if T > FP8_STAGED_ROWS:
         a, scales, kind = scratch[codes], scratch[scales_at], _X_CODES
         _run("sharpi_fp8_rows", scratch[h], _BF16, a, scales, rows, stride, 0, 0.0, stream)
     _run("sharpi_fp8_few_sum", a, scales, kind, w2.codes.data_ptr(), w2.scales.data_ptr(), w2.stored_rows, out.data_ptr(), ids_at, w_out, T, k, E,
-         also, N, stride, SUM_TILES, shares, scratch[part], scratch[counters], stream)
+         also, N, stride, shares, scratch[part], scratch[counters], stream)
     return out
-
-
-SUM_TILES = 2        # half tiles of 16 columns a block of the sum takes
 
 
 def sum_shares(tiles: int, blocks: int, units: int) -> int:
@@ -438,7 +449,8 @@ def sum_shares(tiles: int, blocks: int, units: int) -> int:
 
 def feed_forward_fp8(x: Union[torch.Tensor, Fp8Rows], w_gate_up: Fp8Weight, w_down: Fp8Weight, act=ACT_SILU) -> torch.Tensor:
     """A gated feed-forward in 8 bits: h = act(g) * u with (g | u) = x W_gate_up^T, rounded to bfloat16 and quantised again, then h W_down^T: bfloat16
-    [M, N].  A few rows: two launches (up to 16 rows of bfloat16; four up to 64); more: the quantised h is the first product's epilogue."""
+    [M, N].  Up to 64 rows by streaming the weights, in two launches (up to two rows of bfloat16) to four; more rows: the quantised h is the first product's
+    epilogue."""
     M, K, inner, N = _layer_checked(x, w_gate_up, w_down, 2, "feed_forward_fp8")
     code, limit = _known_act_pair(act)
     with _device_of(w_down.codes):
@@ -465,10 +477,10 @@ def experts_fp8(x: Union[torch.Tensor, Fp8Rows], ids: torch.Tensor, wts: torch.T
     """A layer of routed experts in 8 bits, whole: out[t] = sum_j wts[t, j] F_e(x[t]) over the token's picks e = ids[t, j], with F_e the gated
     feed-forward of matrix e (see ``feed_forward_fp8``); with ``score_on_input`` the pick's score multiplies g and u instead.  ``shared``: the stacks hold
     one more matrix behind the experts, whose feed-forward of every token is added.  ids int32 [T, k] and wts float32 [T, k] as the router
-    gives them (``router_topk``); a pick of the experts' number or above adds nothing, negative ones are not allowed.  bfloat16 [T, N].
+    gives them (``router_topk``); a pick outside 0 .. E - 1 adds nothing.  bfloat16 [T, N].
 
-    Up to 64 tokens the picks are taken as they are: two launches for up to 16 rows of bfloat16 (four beyond), the second of which adds the experts' outputs in float.  More
-    tokens are sorted by expert."""
+    Up to 16 tokens the picks are taken as they are and the weights streamed, in two launches (up to two rows of bfloat16) to four, the last of which adds
+    the experts' outputs.  More tokens (up to 4 GB of codes) are sorted by expert; their outputs are kept in float until they are added."""
     T, K, inner, N = _layer_checked(x, w_gate_up, w_down, 3, "experts_fp8")
     _dev(ids, wts)
     _i32(ids, "ids")
@@ -476,7 +488,7 @@ def experts_fp8(x: Union[torch.Tensor, Fp8Rows], ids: torch.Tensor, wts: torch.T
           "experts_fp8: ids must be int32 and wts float32 [T, k]")
     _same_device(w_down.codes, ids, wts)
     E, k = w_gate_up.shape[0] - (1 if shared else 0), ids.shape[1]
-    _need(0 < E <= FP8_MAX_EXPERTS and k <= FP8_FEW_PAIRS, f"experts_fp8: up to {FP8_MAX_EXPERTS} experts and {FP8_FEW_PAIRS} picks")
+    _need(0 < E <= FP8_MAX_EXPERTS and k <= FP8_FEW_PAIRS and T * (k + 1) < 1 << 31, f"experts_fp8: up to {FP8_MAX_EXPERTS} experts and {FP8_FEW_PAIRS} picks")
     code, limit = _known_act_pair(act)
     with _device_of(w_down.codes):
         if T == 0:

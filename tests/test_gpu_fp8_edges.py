@@ -1,0 +1,130 @@
+"""8-bit operators at the ends of their ranges: picks of no expert, most experts and picks, rows far apart in memory, operands at odd addresses."""
+import pytest
+import torch
+
+import plain_fp8 as plain
+from test_gpu_fp8 import DEV, _gen, _layer, _layer_want, _normal, _picks, _weight, _whole
+
+pytestmark = pytest.mark.gpu
+
+
+def _close(y, want, bound):
+    assert ((y.double() - want).abs() <= bound + 2 ** -20 * want.abs() + plain.stored(want)).all()
+
+
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("T", [1, 3, 16, 40, 700])
+def test_tokens_whose_picks_are_of_no_expert(T, shared):
+    """A padded batch: every pick -1, or the experts' number, of some tokens or of all."""
+    from sharpinference_amd import ops
+    g = _gen(T)
+    E, k = 5, 3
+    x = _whole(g, T, 256).bfloat16()
+    w1, w2, p1, p2 = _layer(g, E, 256, 96, 70, shared)
+    ids, wts = _picks(g, T, E, k)
+    for none in (-1, E, -(1 << 31), (1 << 31) - 1):
+        for rows in (slice(T // 2, None), slice(None)):
+            some = ids.clone()
+            some[rows] = none
+            for on_input in (False, True):
+                y = ops.experts_fp8(x, some, wts, p1, p2, score_on_input=on_input, shared=shared)
+                _close(y, *_layer_want(x, some, wts, w1, w2, "silu", on_input, shared))
+                assert shared or (y[rows] == 0).all()
+
+
+@pytest.mark.parametrize("T", [1, 2, 4, 16, 30])
+def test_one_expert_for_every_pick(T):
+    from sharpinference_amd import ops
+    g = _gen(T)
+    E, k = 6, 5
+    x = _whole(g, T, 384).bfloat16()
+    w1, w2, p1, p2 = _layer(g, E, 384, 130, 40, False)
+    ids, wts = torch.full((T, k), 4, dtype=torch.int32, device=DEV), torch.rand(T, k, generator=g, device=DEV)
+    _close(ops.experts_fp8(x, ids, wts, p1, p2), *_layer_want(x, ids, wts, w1, w2, "silu", False, False))
+
+
+@pytest.mark.parametrize("T,E,k", [(1, 1023, 512), (2, 1023, 8), (16, 1023, 32), (16, 40, 33), (40, 1023, 8), (20, 700, 512), (5, 1, 1)])
+def test_most_experts_and_most_picks(T, E, k):
+    from sharpinference_amd import ops
+    g = _gen(T, E, k)
+    x = _whole(g, T, 128).bfloat16()
+    w1, w2, p1, p2 = _layer(g, E, 128, 32, 16, True)
+    ids, wts = _picks(g, T, E, k)
+    want, bound, wide = (torch.zeros(T, 16, dtype=torch.float64, device=DEV) for _ in range(3))
+    for e in range(E + 1):
+        at, pick = torch.nonzero(ids == e, as_tuple=True) if e < E else (torch.arange(T, device=DEV), None)
+        if at.numel():
+            y, d = plain.feed_forward(x[at].double(), w1[e].double(), plain.rows(w2[e]), "silu", None)
+            f = 1.0 if pick is None else wts[at, pick, None].double()
+            want.index_add_(0, at, y * f)
+            bound.index_add_(0, at, d * f)
+            wide.index_add_(0, at, (y * f).abs())              # (each of the k + 1 sums in float: half a step of what has come together)
+    y = ops.experts_fp8(x, ids, wts, p1, p2, shared=True)
+    assert ((y.double() - want).abs() <= bound + (k + 1) * 2 ** -24 * wide + plain.stored(want)).all()
+
+
+@pytest.mark.parametrize("T,k", [(1500, 2), (5000, 4), (9000, 3)])
+def test_many_tokens_some_without_an_expert(T, k):
+    """Every form of the sorted list, with picks that have no row."""
+    from sharpinference_amd import ops
+    g = _gen(T, k)
+    x = _whole(g, T, 128).bfloat16()
+    w1, w2, p1, p2 = _layer(g, 7, 128, 64, 48, False)
+    ids = torch.randint(-1, 8, (T, k), generator=g, device=DEV).int()
+    wts = torch.rand(T, k, generator=g, device=DEV)
+    _close(ops.experts_fp8(x, ids, wts, p1, p2), *_layer_want(x, ids, wts, w1, w2, "silu", False, False))
+
+
+def test_more_rows_than_a_launch_has_blocks_across():
+    from sharpinference_amd import ops
+    M = (1 << 24) + 37
+    x = torch.randint(-500, 500, (M, 8), generator=_gen(1), device=DEV).bfloat16()
+    q = ops.quantize_rows(x)
+    for at in (0, (1 << 24) - 20, M - 50):
+        want = ops.quantize_rows(x[at:at + 50])
+        assert torch.equal(q.codes[at:at + 50].view(torch.uint8), want.codes.view(torch.uint8)) and torch.equal(q.scales[at:at + 50], want.scales)
+
+
+def test_rows_behind_four_gigabytes():
+    """Tiles reach rows at any distance; a gather of rows that far apart is refused."""
+    from sharpinference_amd import ops
+    g = _gen(2)
+    K, M = 65536, 66000
+    w, p = _weight(g, 40, K)
+    x = torch.empty(M, K, dtype=torch.bfloat16, device=DEV)
+    x[:-300] = 1.0
+    x[-300:] = _normal(g, 300, K).bfloat16()
+    q = ops.quantize_rows(x)
+    y = ops.linear_fp8(q, p)
+    del x
+    a, b = ops.Fp8Rows(q.codes[-300:], q.scales[-300:], K).values().double(), plain.rows(w)
+    want = a @ b.T
+    assert ((y[-300:].double() - want).abs() <= plain.cut(a, b) + plain.stored(want)).all()
+    one, two = ops.quantize_weight(_normal(g, 1, 2, K), True), ops.quantize_weight(_normal(g, 1, 4, 1))
+    ids, wts = torch.zeros(M, 1, dtype=torch.int32, device=DEV), torch.ones(M, 1, device=DEV)
+    with pytest.raises(ops.KernelError):
+        ops.experts_fp8(q, ids, wts, one, two)
+
+
+def _moved(t, by):
+    room = torch.empty(t.numel() + by, dtype=torch.uint8, device=DEV)
+    room[by:] = t.view(torch.uint8).flatten()
+    return room[by:].view(t.dtype).view(t.shape)
+
+
+@pytest.mark.parametrize("M", [3, 100])
+def test_codes_and_scales_at_odd_addresses(M):
+    """Refused, or the same result."""
+    from sharpinference_amd import ops
+    g = _gen(M)
+    _, w = _weight(g, 64, 256)
+    q = ops.quantize_rows(_normal(g, M, 256).bfloat16())
+    want = ops.linear_fp8(q, w)
+    with pytest.raises(ops.KernelError):
+        ops.linear_fp8(ops.Fp8Rows(_moved(q.codes, 4), q.scales, 256), w)
+    off = ops.Fp8Rows(q.codes, _moved(q.scales, 1), 256)
+    if M <= 64:
+        assert torch.equal(ops.linear_fp8(off, w), want)
+    else:
+        with pytest.raises(ops.KernelError):
+            ops.linear_fp8(off, w)
