@@ -6,6 +6,31 @@
 // reaches; a row of 5,120: the launch.
 #include "fp8.h"
 
+// Eight values of a block whose others 15 neighbouring lanes hold: their codes, and the block's byte.
+__device__ __forceinline__ int eight_codes(const float (&v)[8], uint32_t (&c)[2]) {
+  uint32_t top = 0;
+  bool bad[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t m = __float_as_uint(v[i]) & 0x7fffffffu;
+    bad[i] = m >= 0x7f800000u;
+    if (!bad[i] && m > top) top = m;
+  }
+  float t = __uint_as_float(top);
+  t = fmaxf(t, row_rotated<8>(t));
+  t = fmaxf(t, row_rotated<4>(t));
+  t = fmaxf(t, row_rotated<2>(t));
+  t = fmaxf(t, row_rotated<1>(t));
+  const int s = f8_scale_of(__float_as_uint(t));
+  const float scale = f8_scale_value(s);
+  c[0] = f8_codes4(v[0], v[1], v[2], v[3], scale);
+  c[1] = f8_codes4(v[4], v[5], v[6], v[7], scale);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (bad[i]) c[i / 4] = (c[i / 4] & ~(0xffu << (i % 4 * 8))) | kF8Nan << (i % 4 * 8);
+  return s;
+}
+
 // WIDE: rows of whole runs of eight from 16-byte addresses; else element by element.
 template <typename T, bool GATED, bool WIDE>
 __global__ __launch_bounds__(256) void fp8_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
@@ -40,25 +65,8 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const T* __restrict__ x, 
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = to_f32(from_f32<T>(gated_f32(act, v[i], w[i], 1.f, false)));
   }
-  uint32_t top = 0;
-  bool bad[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t m = __float_as_uint(v[i]) & 0x7fffffffu;
-    bad[i] = m >= 0x7f800000u;
-    if (!bad[i] && m > top) top = m;
-  }
-  float t = __uint_as_float(top);
-  t = fmaxf(t, row_rotated<8>(t));
-  t = fmaxf(t, row_rotated<4>(t));
-  t = fmaxf(t, row_rotated<2>(t));
-  t = fmaxf(t, row_rotated<1>(t));
-  const int s = f8_scale_of(__float_as_uint(t));
-  const float scale = f8_scale_value(s);
-  uint32_t c[2] = {f8_codes4(v[0], v[1], v[2], v[3], scale), f8_codes4(v[4], v[5], v[6], v[7], scale)};
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (bad[i]) c[i / 4] = (c[i / 4] & ~(0xffu << (i % 4 * 8))) | kF8Nan << (i % 4 * 8);
+  uint32_t c[2];
+  const int s = eight_codes(v, c);
   *reinterpret_cast<uint2*>(codes + b * kF8Block + l * 8) = make_uint2(c[0], c[1]);
   if (l == 0) scales[row * su + u] = (uint8_t)s;
   else if (u == U - 1 && U - 1 + l < su) scales[row * su + U - 1 + l] = 127;      // (the bytes behind the last block: a scale of one)
@@ -84,6 +92,60 @@ SHARPI_EXPORT int sharpi_fp8_rows(const void* x, int dtype, void* codes, void* s
   else return SHARPI_ERR_ARG;
 #undef FR_FORM
 #undef FR
+  SHARPI_CHECK_LAUNCH();
+  return SHARPI_OK;
+}
+
+// Matrices [N, K] (GATED: gate rows, then as many up rows) into the stored order of tiles, each in one pass.  16 lanes hold a block of 128 as above; a block
+// of threads takes 16 rows of a tile, so that a run of 256 bytes of the stored order is written at a time.  Bound: a pass over memory; run when a
+// program loads its weights.
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(256) void fp8_weight_kernel(const T* __restrict__ w, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int N, int K, int U,
+                                                         int stored, int gated) {
+  const int l = threadIdx.x & 15, U4 = (U + 3) >> 2, half = blockIdx.x & 1;
+  const int u = (blockIdx.x >> 1) % U, tile = (blockIdx.x >> 1) / U, r = half * 16 + (threadIdx.x >> 4);
+  const size_t e = blockIdx.y, at = e * (stored / kF8Tile) + tile;
+  // the row of the matrix that is stored there (each half of a gated one is filled up by itself), if one is
+  const int part = gated ? stored / 2 : stored, mine = gated ? N / 2 : N, row = tile * kF8Tile + r, in = row % part;
+  const bool real = in < mine;
+  const T* src = w + (e * N + (row / part) * mine + in) * K;
+  const int k = u * kF8Block + l * 8;
+  float v[8];
+  if constexpr (WIDE) {
+    if (real && k < K) load8(src + k, v);
+    else
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = real && k + i < K ? to_f32(src[k + i]) : 0.f;
+  }
+  uint32_t c[2];
+  const int s = eight_codes(v, c);
+  // k = 64 s + 32 g + 16 p + byte: lane l has byte 8 (l & 1) of piece l / 2 % 2 of group l / 4 % 2 of half l / 8
+  uint8_t* to = codes + (at * U + u) * kF8TileBytes + (l >> 3) * 2048 + (l >> 1 & 1) * 1024 + (l >> 2 & 1) * 512 + r * 16 + (l & 1) * 8;
+  *reinterpret_cast<uint2*>(to) = make_uint2(c[0], c[1]);
+  uint8_t* byte = scales + (at * U4 + (u >> 2)) * 128 + r * 4;
+  if (l == 0) byte[u & 3] = real ? (uint8_t)s : 127;
+  else if (u == U - 1 && (u & 3) + l < 4) byte[(u & 3) + l] = 127;
+}
+
+// codes, scales: of `matrices` of them, each of f8_padded_rows(N) stored rows (gated: twice those of N / 2).
+SHARPI_EXPORT int sharpi_fp8_weight(const void* w, int dtype, void* codes, void* scales, int matrices, int N, int K, int gated, hipStream_t stream) {
+  if (matrices <= 0) return SHARPI_OK;
+  if (N <= 0 || K <= 0 || K >= kF8MostK || (gated && N % 2) || matrices > 0xffff) return SHARPI_ERR_ARG;
+  const int U = f8_blocks(K), stored = gated ? 2 * f8_padded_rows(N / 2) : f8_padded_rows(N);
+  const long long blocks = (long long)stored / kF8Tile * U * 2;
+  if (blocks > 0xffffff) return SHARPI_ERR_ARG;             // (of 256 threads each, of which a launch has at most 2^32 along x)
+  const dim3 grid((unsigned)blocks, (unsigned)matrices), block(256);
+  const bool wide = K % 8 == 0 && ((uintptr_t)w & 15) == 0;
+#define FW_FORM(T)                                                                                                                                \
+  if (wide) fp8_weight_kernel<T, true><<<grid, block, 0, stream>>>((const T*)w, (uint8_t*)codes, (uint8_t*)scales, N, K, U, stored, gated);  \
+  else fp8_weight_kernel<T, false><<<grid, block, 0, stream>>>((const T*)w, (uint8_t*)codes, (uint8_t*)scales, N, K, U, stored, gated);
+  if (dtype == DT_BF16) { FW_FORM(bf16_t) }
+  else if (dtype == DT_F32) { FW_FORM(float) }
+  else return SHARPI_ERR_ARG;
+#undef FW_FORM
   SHARPI_CHECK_LAUNCH();
   return SHARPI_OK;
 }

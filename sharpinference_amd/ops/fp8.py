@@ -162,16 +162,22 @@ class Fp8Weight:
 
 
 def _pack(codes: torch.Tensor, scales: torch.Tensor, gated: bool, dst_codes: torch.Tensor, dst_scales: torch.Tensor) -> None:
-    """One matrix: codes uint8 [N, K], scales uint8 [N, blocks], into the stored order."""
-    (N, K), U = codes.shape, scales.shape[1]
-    R, U4 = dst_codes.shape[0] * FP8_TILE, dst_scales.shape[1]
-    rows, bytes_ = codes.new_zeros(R, U * FP8_BLOCK), scales.new_full((R, U4 * 4), 127)
-    for src, dst, n in ((0, 0, N // 2), (N // 2, R // 2, N // 2)) if gated else ((0, 0, N),):
-        rows[dst:dst + n, :K].copy_(codes[src:src + n])
-        bytes_[dst:dst + n, :U].copy_(scales[src:src + n])
-    # [tile, row, block, half, group, piece, 16] -> [tile, block, half, piece, group, row, 16]
-    dst_codes.view(R // 32, U, 2, 2, 2, 32, 16).copy_(rows.view(R // 32, 32, U, 2, 2, 2, 16).permute(0, 2, 3, 5, 4, 1, 6))
-    dst_scales.copy_(bytes_.view(R // 32, 32, U4, 4).permute(0, 2, 1, 3))
+    """Matrices: codes uint8 [E, N, K], scales uint8 [E, N, blocks], into the stored order."""
+    (E, N, K), U = codes.shape, scales.shape[2]
+    R, U4 = dst_codes.shape[1] * FP8_TILE, dst_scales.shape[2]
+    halves = ((0, 0, N // 2), (N // 2, R // 2, N // 2)) if gated else ((0, 0, N),)
+    rows, bytes_ = codes.contiguous(), scales
+    if R != N or K != U * FP8_BLOCK or rows.data_ptr() % 8:
+        rows = codes.new_zeros(E, R, U * FP8_BLOCK)
+        for src, dst, n in halves:
+            rows[:, dst:dst + n, :K].copy_(codes[:, src:src + n])
+    if R != N or U != U4 * 4:
+        bytes_ = scales.new_full((E, R, U4 * 4), 127)
+        for src, dst, n in halves:
+            bytes_[:, dst:dst + n, :U].copy_(scales[:, src:src + n])
+    # [tile, row, block, half, group, piece, 16] -> [tile, block, half, piece, group, row, 16], the 16 bytes as two words
+    dst_codes.view(torch.int64).view(E, R // 32, U, 2, 2, 2, 32, 2).copy_(rows.view(torch.int64).view(E, R // 32, 32, U, 2, 2, 2, 2).permute(0, 1, 3, 4, 6, 5, 2, 7))
+    dst_scales.copy_(bytes_.reshape(E, R // 32, 32, U4, 4).permute(0, 1, 3, 2, 4))
 
 
 def _new_weight(shape, gated: bool, device) -> Fp8Weight:
@@ -195,10 +201,12 @@ def fp8_weight(codes: torch.Tensor, scales: torch.Tensor, gated: bool = False) -
           "fp8_weight: scales must be uint8, one for each row's block of 128, beside the codes")
     w = _new_weight(tuple(codes.shape), gated, codes.device)
     if codes.dim() == 2:
-        _pack(codes.view(torch.uint8), scales, gated, w.codes, w.scales)
-    else:
-        for e in range(codes.shape[0]):
-            _pack(codes[e].view(torch.uint8), scales[e], gated, w.codes[e], w.scales[e])
+        _pack(codes.view(torch.uint8)[None], scales[None], gated, w.codes[None], w.scales[None])
+        return w
+    at_once = max(1, (1 << 30) // (w.stored_rows * _blocks(codes.shape[2]) * FP8_BLOCK))      # (matrices: what is filled up is a copy of them)
+    for e in range(0, codes.shape[0], at_once):
+        some = slice(e, e + at_once)
+        _pack(codes[some].view(torch.uint8), scales[some], gated, w.codes[some], w.scales[some])
     return w
 
 
@@ -210,20 +218,22 @@ def empty_fp8_weight(shape, gated: bool, device) -> Fp8Weight:
 def quantize_into(dst: Fp8Weight, w: torch.Tensor) -> None:
     """A bfloat16 or float32 matrix on the GPU, quantised (``quantize_rows`` of its rows) into dst [N, K] of its shape."""
     _need(dst.dim() == 2 and tuple(w.shape) == dst.shape and w.device == dst.device, f"quantize_into: a matrix {dst.shape} on the destination's device is wanted")
-    q = quantize_rows(w.contiguous())
-    K = w.shape[1]
-    _pack(q.codes.view(torch.uint8)[:, :K], q.scales[:, :_blocks(K)], dst.gated, dst.codes, dst.scales)
+    _quantize(dst, w)
+
+
+def _quantize(dst: Fp8Weight, w: torch.Tensor) -> None:
+    w = w.contiguous()
+    _dev(w, dst.codes)
+    with _device_of(w):
+        _run("sharpi_fp8_weight", w.data_ptr(), _code(w.dtype), dst.codes.data_ptr(), dst.scales.data_ptr(), 1 if w.dim() == 2 else w.shape[0], *w.shape[-2:],
+             int(dst.gated), _stream_of(w))
 
 
 def quantize_weight(w: torch.Tensor, gated: bool = False) -> Fp8Weight:
     """A bfloat16 or float32 matrix [(E,) N, K] on the GPU in 8 bits, in the kernels' order."""
     _need(w.is_cuda and w.dim() in (2, 3), "quantize_weight: a matrix [N, K] or a stack [E, N, K] on the GPU")
     out = _new_weight(tuple(w.shape), gated, w.device)
-    if w.dim() == 2:
-        quantize_into(out, w)
-    else:
-        for e in range(w.shape[0]):
-            quantize_into(out.select(e), w[e])
+    _quantize(out, w)
     return out
 
 

@@ -34,6 +34,7 @@ _SIGNATURES = {
     "sharpi_attention_decode_values": [P, P, P, P, P, P, P, P, P, P, I, I, F, I, I, I, I, I, I, I, I, I, F, I, P, I, P, I, P],
     "sharpi_attention_prefill": [P, P, P, P, P, P, P, I, I, I, I, F, I, I, I, I, I, I, I, F, I, P, I, P, I, P],
     "sharpi_fp8_rows": [P, I, P, P, I, I, I, F, P],
+    "sharpi_fp8_weight": [P, I, P, P, I, I, I, I, P],
     "sharpi_fp8_few": [P, P, I, P, P, I, P, I, I, I, I, P],
     "sharpi_fp8_few_gated": [P, P, I, P, P, I, P, I, P, P, I, I, I, I, I, I, I, F, P, I, P],
     "sharpi_fp8_few_sum": [P, P, I, P, P, I, P, P, P, I, I, I, I, I, I, I, P, P, P],

@@ -12,6 +12,11 @@ def test_matrices_beyond_the_largest():
             ops.empty_fp8_weight(shape, False, "cpu")
 
 
+def test_matrices_of_the_host_are_not_quantised():
+    with pytest.raises(ops.KernelError, match="live on the GPU"):
+        ops.quantize_into(ops.empty_fp8_weight((4, 128), False, "cpu"), torch.zeros(4, 128))
+
+
 @pytest.mark.parametrize("gated", [False, True])
 def test_a_matrix_of_parts_that_do_not_fit(gated):
     w = ops.empty_fp8_weight((3, 66, 300), gated, "cpu")

@@ -75,6 +75,25 @@ def test_many_tokens_some_without_an_expert(T, k):
     _close(ops.experts_fp8(x, ids, wts, p1, p2), *_layer_want(x, ids, wts, w1, w2, "silu", False, False))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("shape", [(2, 8), (34, 136), (66, 1000), (130, 4096), (3, 70, 261), (5, 64, 520)])
+def test_matrices_are_quantised_as_their_rows_are(shape, gated, dtype):
+    """Aligned and not, filled up and whole, one and a stack: what the rows' kernel gives, in the stored order."""
+    from sharpinference_amd import ops
+    K = shape[-1]
+    room = _normal(_gen(*shape), torch.Size(shape).numel() + 3).to(dtype)
+    room[5] = float("inf")
+    for w in (room[:-3].view(shape), room[3:].view(shape), room[:-3].view(*shape[:-2], K, shape[-2]).transpose(-1, -2)):
+        q = ops.quantize_rows(w.reshape(-1, K).contiguous())
+        U = -(-K // 128)
+        want = ops.fp8_weight(q.codes[:, :K].reshape(shape), q.scales[:, :U].reshape(*shape[:-1], U), gated)
+        got = ops.quantize_weight(w, gated)
+        assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
+    with pytest.raises(ops.KernelError):
+        ops.quantize_weight(room[:-3].view(shape).half(), gated)
+
+
 def test_more_rows_than_a_launch_has_blocks_across():
     from sharpinference_amd import ops
     M = (1 << 24) + 37
