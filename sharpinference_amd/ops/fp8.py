@@ -406,10 +406,12 @@ def tile_fp8(M: int, N: int, K: int, gated: bool, units: int) -> Tuple[int, int,
     return min(((h, nt, s) for h, nt in choices for s in range(1, most + 1)), key=lambda c: expected(*c))
 
 
-def grouped_tile_fp8(rows: int, groups: int) -> int:
-    """Rows of the tiles of a layer's products at most: in pairs of blocks a unit where an expert has few (us, tiles of 128 and of 256: 64 experts of 2 x 1,408 x
-    2,048, 94 rows each 118 and 123; 16 of 5,120 x 8,192, 6 rows each 125 and 139, 128 rows each 223 and 205, their first product 357 and 326)."""
-    return 128 if rows <= 96 * groups else 256
+def grouped_tile_fp8(K: int) -> int:
+    """Rows of the tiles of a layer's products at most: over a short k in pairs of blocks a unit, which fill each other's gaps at a tile's start and end (us, tiles of
+    128 and of 256: 64 experts of 2 x 1,408 x 2,048, 94 rows each 100 and 105, 188 146 and 150; 128 of 2 x 768 x 2,048, 125 rows 125 and 132; 16 of 16,384 x 5,120, 38 rows
+    262 and 241, 128 357 and 331; 32 of 5,760 x 2,880, 38 rows 125 and 112, 375 326 and 301).  Of 72 launches timed both ways those it
+    chooses take 1.7 % more than the faster ones in the mean (always 256: 3.7 %)."""
+    return 128 if K <= 2048 else 256
 
 
 def _layer_checked(x, w_gate_up: Fp8Weight, w_down: Fp8Weight, dims: int, who: str):
@@ -520,14 +522,14 @@ def _many_layer(x, ids, wts, w1: Fp8Weight, w2: Fp8Weight, code: int, limit: flo
     shared_y = y + n * N * 4
     scratch.make(dev)
     out = torch.empty((T, N), dtype=torch.bfloat16, device=dev)
-    stream, height = _stream_of(out), grouped_tile_fp8(n, E)
+    stream, K = _stream_of(out), w1.shape[-1]
     a, a_scales, _ = operand.ready(scratch, stream)
     _run("sharpi_moe_permute", ids.data_ptr(), wts.data_ptr(), scratch[offsets], scratch[tokens], scratch[scores], scratch[inv_pos], None, 0,
          T, k, E, 0, 1, stream)
     _run("sharpi_fp8_tiles_gated", a, a_scales, T, w1.codes.data_ptr(), w1.scales.data_ptr(), w1.stored_rows, scratch[codes], scratch[scales],
-         n, inner, w1.shape[-1], scratch[tokens], scratch[offsets], E, along, scratch[scores] if on_input else None, code, limit, height, stream)
+         n, inner, K, scratch[tokens], scratch[offsets], E, along, scratch[scores] if on_input else None, code, limit, grouped_tile_fp8(K), stream)
     _run("sharpi_fp8_tiles", scratch[codes], scratch[scales], n + along, w2.codes.data_ptr(), w2.scales.data_ptr(), w2.stored_rows, scratch[y], _F32, n, N, inner,
-         None, scratch[offsets], E, along, height, 2, 1, stream)
+         None, scratch[offsets], E, along, grouped_tile_fp8(inner), 2, 1, stream)
     _run("sharpi_fp8_combine", scratch[y], scratch[inv_pos], ids.data_ptr(), scratch[shared_y] if shared else None, None if on_input else wts.data_ptr(),
          out.data_ptr(), T, N, k, E, stream)
     return out
