@@ -31,8 +31,20 @@ __device__ __forceinline__ int eight_codes(const float (&v)[8], uint32_t (&c)[2]
   return s;
 }
 
-// WIDE: rows of whole runs of eight from 16-byte addresses; else element by element.
-template <typename T, bool GATED, bool WIDE>
+// Eight values from a row's k on (zeros behind its K), in loads of 16 bytes at whatever address: the memory takes any.
+template <typename T> __device__ __forceinline__ void load_eight(const T* __restrict__ row, int k, int K, float (&v)[8]) {
+  if (k + 8 <= K) {
+    T t[8];
+    __builtin_memcpy(t, row + k, sizeof(t));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(t[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_f32(row[k + i]) : 0.f;
+  }
+}
+
+template <typename T, bool GATED>
 __global__ __launch_bounds__(256) void fp8_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                                                        long long n_blocks, int K, int U, int su, GatedAct act) {
   const long long b = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * 16 + (threadIdx.x >> 4);
@@ -40,28 +52,12 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const T* __restrict__ x, 
   const int l = threadIdx.x & 15;
   const long long row = b / U;
   const int u = (int)(b - row * U), k = u * kF8Block + l * 8;
-  const T* src = x + row * (GATED ? 2 * (long long)K : K) + k;
+  const T* src = x + row * (GATED ? 2 * (long long)K : K);
   float v[8];
-  if constexpr (WIDE) {
-    if (k < K) load8(src, v);
-    else
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_f32(src[i]) : 0.f;
-  }
+  load_eight(src, k, K, v);
   if constexpr (GATED) {
     float w[8];
-    if constexpr (WIDE) {
-      if (k < K) load8(src + K, w);
-      else
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = 0.f;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = k + i < K ? to_f32(src[K + i]) : 0.f;
-    }
+    load_eight(src + K, k, K, w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = to_f32(from_f32<T>(gated_f32(act, v[i], w[i], 1.f, false)));
   }
@@ -82,15 +78,10 @@ SHARPI_EXPORT int sharpi_fp8_rows(const void* x, int dtype, void* codes, void* s
   const long long blocks = (n + 15) / 16, across = blocks < 1 << 20 ? blocks : 1 << 20;      // (a launch has at most 2^32 threads along x)
   if ((blocks + across - 1) / across > 0xffff) return SHARPI_ERR_ARG;
   const dim3 grid((unsigned)across, (unsigned)((blocks + across - 1) / across)), block(256);
-  const bool wide = K % 8 == 0 && ((uintptr_t)x & 15) == 0;
-#define FR(T, G, W) fp8_rows_kernel<T, G, W><<<grid, block, 0, stream>>>((const T*)x, (uint8_t*)codes, (uint8_t*)scales, n, K, U, su, ga)
-#define FR_FORM(T)                                   \
-  if (act) { if (wide) FR(T, true, true); else FR(T, true, false); } \
-  else { if (wide) FR(T, false, true); else FR(T, false, false); }
-  if (dtype == DT_BF16) { FR_FORM(bf16_t) }
-  else if (dtype == DT_F32) { FR_FORM(float) }
+#define FR(T, G) fp8_rows_kernel<T, G><<<grid, block, 0, stream>>>((const T*)x, (uint8_t*)codes, (uint8_t*)scales, n, K, U, su, ga)
+  if (dtype == DT_BF16) { if (act) FR(bf16_t, true); else FR(bf16_t, false); }
+  else if (dtype == DT_F32) { if (act) FR(float, true); else FR(float, false); }
   else return SHARPI_ERR_ARG;
-#undef FR_FORM
 #undef FR
   SHARPI_CHECK_LAUNCH();
   return SHARPI_OK;
@@ -99,7 +90,7 @@ SHARPI_EXPORT int sharpi_fp8_rows(const void* x, int dtype, void* codes, void* s
 // Matrices [N, K] (GATED: gate rows, then as many up rows) into the stored order of tiles, each in one pass.  16 lanes hold a block of 128 as above; a block
 // of threads takes 16 rows of a tile, so that a run of 256 bytes of the stored order is written at a time.  Bound: a pass over memory; run when a
 // program loads its weights.
-template <typename T, bool WIDE>
+template <typename T>
 __global__ __launch_bounds__(256) void fp8_weight_kernel(const T* __restrict__ w, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int N, int K, int U,
                                                          int stored, int gated) {
   const int l = threadIdx.x & 15, U4 = (U + 3) >> 2, half = blockIdx.x & 1;
@@ -111,15 +102,7 @@ __global__ __launch_bounds__(256) void fp8_weight_kernel(const T* __restrict__ w
   const T* src = w + (e * N + (row / part) * mine + in) * K;
   const int k = u * kF8Block + l * 8;
   float v[8];
-  if constexpr (WIDE) {
-    if (real && k < K) load8(src + k, v);
-    else
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = real && k + i < K ? to_f32(src[k + i]) : 0.f;
-  }
+  load_eight(src, real ? k : K, K, v);
   uint32_t c[2];
   const int s = eight_codes(v, c);
   // k = 64 s + 32 g + 16 p + byte: lane l has byte 8 (l & 1) of piece l / 2 % 2 of group l / 4 % 2 of half l / 8
@@ -138,14 +121,11 @@ SHARPI_EXPORT int sharpi_fp8_weight(const void* w, int dtype, void* codes, void*
   const long long blocks = (long long)stored / kF8Tile * U * 2;
   if (blocks > 0xffffff) return SHARPI_ERR_ARG;             // (of 256 threads each, of which a launch has at most 2^32 along x)
   const dim3 grid((unsigned)blocks, (unsigned)matrices), block(256);
-  const bool wide = K % 8 == 0 && ((uintptr_t)w & 15) == 0;
-#define FW_FORM(T)                                                                                                                                \
-  if (wide) fp8_weight_kernel<T, true><<<grid, block, 0, stream>>>((const T*)w, (uint8_t*)codes, (uint8_t*)scales, N, K, U, stored, gated);  \
-  else fp8_weight_kernel<T, false><<<grid, block, 0, stream>>>((const T*)w, (uint8_t*)codes, (uint8_t*)scales, N, K, U, stored, gated);
-  if (dtype == DT_BF16) { FW_FORM(bf16_t) }
-  else if (dtype == DT_F32) { FW_FORM(float) }
+#define FW(T) fp8_weight_kernel<T><<<grid, block, 0, stream>>>((const T*)w, (uint8_t*)codes, (uint8_t*)scales, N, K, U, stored, gated)
+  if (dtype == DT_BF16) FW(bf16_t);
+  else if (dtype == DT_F32) FW(float);
   else return SHARPI_ERR_ARG;
-#undef FW_FORM
+#undef FW
   SHARPI_CHECK_LAUNCH();
   return SHARPI_OK;
 }

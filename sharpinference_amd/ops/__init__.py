@@ -2402,5 +2402,5 @@ def delta_chunks(proj: torch.Tensor, c_off: int, conv_w: torch.Tensor, ring: Opt
     return out
 
 
-from .fp8 import (FP8_BLOCK, FP8_FEW_TOKENS, Fp8Rows, Fp8Weight, empty_fp8_weight, experts_fp8, feed_forward_fp8,  # noqa: E402
+from .fp8 import (FP8_BLOCK, FP8_FEW_TOKENS, FP8_MAX_EXPERTS, Fp8Rows, Fp8Weight, empty_fp8_weight, experts_fp8, feed_forward_fp8,  # noqa: E402
                   feed_forwards_are_8_bits, feed_forwards_in_8_bits, fp8_weight, linear_fp8, quantize_into, quantize_rows, quantize_weight)

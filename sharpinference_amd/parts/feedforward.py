@@ -156,7 +156,7 @@ class MoESwiGLU(Part):
     have no tensors and return the layer's input; they take part in the choice (groups, correction) like the others.
     Their share is added where the outputs are summed (``ops.ExpertSum``).
 
-    Loaded under ``ops.feed_forwards_in_8_bits`` gated experts without identity experts beside them, of bfloat16 matrices, are kept
+    Loaded under ``ops.feed_forwards_in_8_bits`` gated experts (up to 1,023) without identity experts beside them, of bfloat16 matrices, are kept
     in 8 bits and run through ``ops.experts_fp8``, a shared expert of their width and activation as one more matrix."""
 
     MERGE_MAX_TOKENS = 16   # one row block of the few-rows kernel for the shared group (measured: up to 64 tokens
@@ -275,7 +275,7 @@ class MoESwiGLU(Part):
         # The experts' matrices are kept only in the order the kernels stream them (no rows: both
         # the few-rows and the many-rows product of the experts read that order), if the sizes allow.
         pack = bf16 and self.inter % 128 == 0 and self.hidden % 128 == 0
-        if bf16 and self.gated and not self.identity and ops.feed_forwards_are_8_bits():
+        if bf16 and self.gated and not self.identity and self.E <= ops.FP8_MAX_EXPERTS and ops.feed_forwards_are_8_bits():
             self._load_8_bits(g, u, d)
             return
         sh_first = None if sh is None else "w_gate_up" if self.gated else "w_up"       # the shared expert's first matrix
