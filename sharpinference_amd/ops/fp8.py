@@ -15,7 +15,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 
-from . import ACT_SILU, _code, _dev, _i32, _known_act_pair, _need, _ptr, _run, compute_units
+from . import ACT_SILU, KernelError, _code, _dev, _i32, _known_act_pair, _need, _ptr, _run, compute_units
 
 FP8_BLOCK = 128                # values that share a scale
 FP8_TILE = 32                  # weight rows of a stored tile
@@ -94,7 +94,8 @@ class _Scratch:
 def _same_device(*ts) -> None:
     first = ts[0].device
     for t in ts:
-        _need(t is None or t.device == first, "operands must live on one device")
+        if t.device != first:
+            raise KernelError("operands must live on one device")
 
 
 class Fp8Rows:
@@ -268,7 +269,8 @@ def quantize_rows(x: torch.Tensor, act=None) -> Fp8Rows:
     code, limit = (0, 0.0) if act is None else _known_act_pair(act)
     _need(not code or x.shape[1] % 2 == 0, "quantize_rows: a gated input is [M, 2I]")
     M, K = x.shape[0], x.shape[1] // (2 if code else 1)
-    _need(K <= FP8_MOST_K and M < 1 << 31, f"quantize_rows: up to {FP8_MOST_K} columns")
+    if K > FP8_MOST_K or M >= 1 << 31:
+        raise KernelError(f"quantize_rows: up to {FP8_MOST_K} columns")
     out = _new_rows(M, K, x.device)
     with _device_of(x):
         _run("sharpi_fp8_rows", x.data_ptr(), dt, out.codes.data_ptr(), out.scales.data_ptr(), M, K, code, limit, _stream_of(x))
@@ -310,7 +312,8 @@ def _rows_checked(x, k: int, who: str) -> None:
     else:
         _dev(x)
         _code(x.dtype)
-    _need(len(x.shape) == 2 and x.shape[1] == k, f"{who}: x {tuple(x.shape)} does not fit weights over {k} columns")
+    if len(x.shape) != 2 or x.shape[1] != k:
+        raise KernelError(f"{who}: x {tuple(x.shape)} does not fit weights over {k} columns")
 
 
 def linear_fp8(x: Union[torch.Tensor, Fp8Rows], w: Fp8Weight) -> torch.Tensor:
@@ -415,10 +418,12 @@ def grouped_tile_fp8(K: int) -> int:
 
 
 def _layer_checked(x, w_gate_up: Fp8Weight, w_down: Fp8Weight, dims: int, who: str):
-    _need(isinstance(w_gate_up, Fp8Weight) and isinstance(w_down, Fp8Weight) and w_gate_up.dim() == w_down.dim() == dims
-          and w_gate_up.gated and not w_down.gated, f"{who}: w_gate_up must be a gated Fp8Weight and w_down a plain one, both {'[E, N, K]' if dims == 3 else '[N, K]'}")
+    if not (isinstance(w_gate_up, Fp8Weight) and isinstance(w_down, Fp8Weight) and w_gate_up.dim() == w_down.dim() == dims
+            and w_gate_up.gated and not w_down.gated):
+        raise KernelError(f"{who}: w_gate_up must be a gated Fp8Weight and w_down a plain one, both {'[E, N, K]' if dims == 3 else '[N, K]'}")
     inner, K = w_gate_up.shape[-2] // 2, w_gate_up.shape[-1]
-    _need(w_down.shape == (*w_gate_up.shape[:-2], w_down.shape[-2], inner), f"{who}: w_gate_up {w_gate_up.shape} and w_down {w_down.shape} do not fit")
+    if w_down.shape != (*w_gate_up.shape[:-2], w_down.shape[-2], inner):
+        raise KernelError(f"{who}: w_gate_up {w_gate_up.shape} and w_down {w_down.shape} do not fit")
     _rows_checked(x, K, who)
     _same_device(w_gate_up.codes, w_down.codes, x if isinstance(x, torch.Tensor) else x.codes)
     return x.shape[0], K, inner, w_down.shape[-2]
@@ -500,7 +505,8 @@ def experts_fp8(x: Union[torch.Tensor, Fp8Rows], ids: torch.Tensor, wts: torch.T
           "experts_fp8: ids must be int32 and wts float32 [T, k]")
     _same_device(w_down.codes, ids, wts)
     E, k = w_gate_up.shape[0] - (1 if shared else 0), ids.shape[1]
-    _need(0 < E <= FP8_MAX_EXPERTS and k <= FP8_FEW_PAIRS and T * (k + 1) < 1 << 31, f"experts_fp8: up to {FP8_MAX_EXPERTS} experts and {FP8_FEW_PAIRS} picks")
+    if not (0 < E <= FP8_MAX_EXPERTS and k <= FP8_FEW_PAIRS and T * (k + 1) < 1 << 31):
+        raise KernelError(f"experts_fp8: up to {FP8_MAX_EXPERTS} experts and {FP8_FEW_PAIRS} picks")
     code, limit = _known_act_pair(act)
     with _device_of(w_down.codes):
         if T == 0:
