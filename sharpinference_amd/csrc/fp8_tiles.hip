@@ -8,9 +8,9 @@
 //
 // Bound: 8,192 x 16,384 x 5,120 takes 540 us, 2.5 PFLOP/s, by power: the matrix cores are busy 74 % of the time at 1.5 GHz, and a loop of that instruction on
 // registers alone runs at 4.8 PFLOP/s.  The library's product in 8 bits (one scale a tensor) reaches 3.0 PFLOP/s at 8,192 x 8,192 x 8,192.
-// Experts of few rows are bound by reading their weights: 16 of 2 x 8,192 x 5,120 with 6 rows each and one always on, 234 us, 6.1 TB/s; 16 with 128 rows each 331 us, 4.1 TB/s
-// of weights and half as much of rows (through L2), and at the start and end of each tile, some 5 us of 80, nothing is on its way.  Their loads begun at
-// other places of k block by block: no change (337).
+// Experts of few rows are bound by reading their weights: 16 of 2 x 8,192 x 5,120 with 6 rows each and one always on, 234 us, 6.1 TB/s.  With more rows the products'
+// power and the memory's add up: a step of a tile of 16, 64, 128 and 256 rows over 5,120 takes 0.73, 0.88, 1.02 and 1.35 us with weights from memory, of 256 rows
+// with weights in the caches 0.88 (16 experts with 128 rows each 331 us, 4.1 TB/s, at 1.9 GHz).  Blocks that begin at places of k of their own: no change (337).
 // Weights straight into registers instead of through LDS: 600 us for the first product above, then at 579.
 #include <type_traits>
 
