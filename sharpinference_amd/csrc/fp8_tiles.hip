@@ -69,10 +69,69 @@ template <bool PAIRED> struct Ring {
   static_assert(scales_at(1) <= scales_at(2) && (PAIRED || (scales_at(3) <= scales_at(2) && scales_at(4) <= scales_at(2))), "the largest ring");
 };
 
+// Gated results near a border of two codes.  The instruction's products are off by some 2e-5 of a sum's rms (fp8.h), now and then by ten times that, which moves 1
+// value in 500 across a border of e4m3, a sixteenth to an eighth of it: nearly as much error in the layer's result as that result's rounding to
+// bfloat16.  Values h that kNear |h| / top of them would move, if they are at least 1 / kNearTop of their block's largest, top (they carry most of the
+// error), are computed once more in float from their rows of codes: about 5 of a tile of 256 x 128, in 4 to 8 us of a tile's 30 to 80 (3,001 rows through
+// 2 x 2,816 x 2,048 53 -> 64 us, 2,048 through 16 experts of 2 x 8,192 x 5,120 and one always on 473 -> 525).  Over 1,700 sizes the layer's error against 64 bits is
+// 1.11 times that of the same sums in float (1.36 at most), without this 1.34 (3.6).  A tile with more than kMost of them (values on borders all
+// along) is left as it is.  The whole product on the bfloat16 instruction would take twice the matrix cores' time.
+constexpr float kNear = 1.5e-4f;
+constexpr float kNearTop = 4.f;
+template <int ROWS> struct F8Near {
+  static constexpr int kMost = 2 * ROWS;
+  int total;
+  unsigned short list[kMost];                  // row of the tile << 7 | column
+};
+// Two columns' products of a row in float, dealt to the wave: x: the row's codes and scales; w: a column's first piece in its tile, ws: its scales.
+// kFlight: pieces of a lane on their way at a time.
+template <int kFlight> __device__ __forceinline__ float2 f8_row_dots(const uint8_t* __restrict__ x, const uint8_t* __restrict__ xs, const uint8_t* __restrict__ w0, const uint8_t* __restrict__ ws0,
+                                              const uint8_t* __restrict__ w1, const uint8_t* __restrict__ ws1, int U) {
+  typedef __attribute__((ext_vector_type(2))) float f32x2;
+  const int lane = threadIdx.x & (kWave - 1), pieces = U * 8;
+  float sum[2] = {0.f, 0.f};
+  for (int p0 = lane; p0 < pieces; p0 += kFlight * kWave) {
+    i32x4 xv[kFlight], wv[2][kFlight];
+    int xb[kFlight], wb[2][kFlight];
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+      const int q = min(p0 + i * kWave, pieces - 1), u = q >> 3, j = q & 7;       // piece j of a block: k = 16 j
+      const size_t at = (size_t)u * kF8TileBytes + (j >> 2) * 2048 + (j & 1) * 1024 + (j >> 1 & 1) * 512;
+      const int byte = (u >> 2) * 128 + (u & 3);
+      xv[i] = *reinterpret_cast<const i32x4*>(x + (size_t)q * 16);
+      wv[0][i] = *reinterpret_cast<const i32x4*>(w0 + at);
+      wv[1][i] = *reinterpret_cast<const i32x4*>(w1 + at);
+      xb[i] = xs[u];
+      wb[0][i] = ws0[byte];
+      wb[1][i] = ws1[byte];
+    }
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+      if (p0 + i * kWave >= pieces) continue;
+      float s[2] = {0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(xv[i][c], false), b = __builtin_amdgcn_cvt_pk_f32_fp8(xv[i][c], true);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const f32x2 d = __builtin_amdgcn_cvt_pk_f32_fp8(wv[t][i][c], false), f = __builtin_amdgcn_cvt_pk_f32_fp8(wv[t][i][c], true);
+          s[t] = fmaf(a[0], d[0], s[t]);
+          s[t] = fmaf(a[1], d[1], s[t]);
+          s[t] = fmaf(b[0], f[0], s[t]);
+          s[t] = fmaf(b[1], f[1], s[t]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) sum[t] = fmaf(s[t] * f8_scale_value(xb[i]), f8_scale_value(wb[t][i]), sum[t]);
+    }
+  }
+  return make_float2(wave_sum(sum[0]), wave_sum(sum[1]));
+}
+
 // One tile: rows row0 .. row_end (up to 64 MT of them) of matrix e against column block nblock.  MT: groups of 32 rows a wave; NT: weight tiles of a wave.
 template <int MT, int NT, bool GATED, bool PAIRED, typename TO>
 __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedAct act, int e, int row0, int row_end, int nblock, unsigned char* smem,
-                                        float (*s_top)[64 * Ring<PAIRED>::kHighest]) {
+                                        float (*s_top)[64 * Ring<PAIRED>::kHighest], F8Near<64 * Ring<PAIRED>::kHighest>* near) {
   using RG = Ring<PAIRED>;
   constexpr int NS = RG::steps(MT), RING = RG::slots(MT) * NS, AHEAD = RING - NS;      // (steps)
   static_assert(NT == 2 || !GATED, "a gated tile's columns are a block of the format");
@@ -312,19 +371,22 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
   } else {
     const int U2 = f8_blocks(o.n_out), su2 = f8_scale_stride(o.n_out);
     float h[MT][16];
+    bool bad = false;                              // (a value of the lane's is not finite)
     auto units = [&](auto code_tag) {              // (the activation is chosen once a tile)
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         const int lrow = (wr * MT + m) * 32 + r, row = min(row0 + lrow, row_end - 1);
         const float sc = o.score != nullptr && sorted ? o.score[row] : 1.f;
-        uint32_t top = 0;
+        uint32_t top = 0, all = 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float v = exists ? bf16_to_f32(f32_to_bf16(f8_unit<decltype(code_tag)::value>(act.limit, acc[0][m][i] * sc, acc[1][m][i] * sc))) : 0.f;
-          const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+          const float v = exists ? f8_unit<decltype(code_tag)::value>(act.limit, acc[0][m][i] * sc, acc[1][m][i] * sc) : 0.f;
+          const uint32_t b = __float_as_uint(bf16_to_f32(f32_to_bf16(v))) & 0x7fffffffu;
           if (b < 0x7f800000u && b > top) top = b;
+          all = b > all ? b : all;
           h[m][i] = v;
         }
+        bad = bad || all >= 0x7f800000u;
         const float t2 = reduce32(__uint_as_float(top), MaxOf{});
         if (g == 0) s_top[wc][lrow] = t2;
       }
@@ -332,6 +394,7 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
     if (act.code == ACT_SWISH_CLAMP) units(std::integral_constant<int, ACT_SWISH_CLAMP>{});
     else if (act.code == ACT_GELU_TANH) units(std::integral_constant<int, ACT_GELU_TANH>{});
     else units(std::integral_constant<int, ACT_SILU>{});
+    if (threadIdx.x == 0) near->total = 0;
     __syncthreads();
     // the codes through LDS, to leave as whole lines: a row's 128 are one block of the format
 #pragma unroll
@@ -339,16 +402,43 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
       const int lrow = (wr * MT + m) * 32 + r;
       const float t = fmaxf(fmaxf(s_top[0][lrow], s_top[1][lrow]), fmaxf(s_top[2][lrow], s_top[3][lrow]));
       const int s = f8_scale_of(__float_as_uint(t));
-      const float scale = f8_scale_value(s);
+      const float scale = f8_scale_value(s), by = t > 0.f ? kNear / t : 0.f;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        uint32_t c = f8_codes4(h[m][4 * q], h[m][4 * q + 1], h[m][4 * q + 2], h[m][4 * q + 3], scale);
+        auto codes_of = [&](float by) {
+          auto moved = [&](int i) { return fmaf(h[m][4 * q + i], fabsf(h[m][4 * q + i]) * by, h[m][4 * q + i]); };
+          return f8_codes4(f32_to_bf16_pair(moved(0), moved(1)), f32_to_bf16_pair(moved(2), moved(3)), scale);
+        };
+        uint32_t c = codes_of(-by);
+        if (const uint32_t differ = c ^ codes_of(by)) {
+          c = codes_of(0.f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if ((__float_as_uint(h[m][4 * q + i]) & 0x7f800000u) == 0x7f800000u) c |= kF8Nan << (8 * i);
+          for (int i = 0; i < 4; ++i)
+            if (const float a = fabsf(h[m][4 * q + i]); (differ >> (8 * i) & 0xff) && a * kNearTop >= t && a <= t * 1.01f && row0 + lrow < row_end) {
+              const int n = atomicAdd(&near->total, 1);
+              if (n < near->kMost) near->list[n] = (unsigned short)(lrow << 7 | (wc * 32 + q * 8 + g * 4 + i));
+            }
+        }
+        if (bad)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if ((__float_as_uint(bf16_to_f32(f32_to_bf16(h[m][4 * q + i]))) & 0x7f800000u) == 0x7f800000u) c |= kF8Nan << (8 * i);
         *reinterpret_cast<uint32_t*>(smem + lrow * 128 + ((wc * 2 + (q >> 1)) ^ (lrow & 7)) * 16 + (q & 1) * 8 + g * 4) = c;
       }
       if (wc == 0 && g == 0 && row0 + lrow < row_end) o.scales[(size_t)(row0 + lrow) * su2 + nblock] = (uint8_t)s;
+    }
+    __syncthreads();
+    const int total = __builtin_amdgcn_readfirstlane(near->total);
+    for (int i = wid; i < total && total <= near->kMost; i += TW) {
+      const int entry = __builtin_amdgcn_readfirstlane(near->list[i]), lrow = entry >> 7, column = entry & 127, row = row0 + lrow, r_at = column & 31;
+      const size_t x_at = x_first + __builtin_amdgcn_readfirstlane(x_row(lrow));
+      const size_t g_at = w_at + block_tile(2 * (column >> 5)), u_at = w_at + block_tile(2 * (column >> 5) + 1);
+      const float2 v = f8_row_dots<PAIRED ? 3 : 6>(p.x + x_at * x_stride, p.xs + x_at * (U4 * 4), p.w + g_at * p.U * kF8TileBytes + r_at * 16, p.ws + g_at * U4 * 128 + r_at * 4,
+                                                   p.w + u_at * p.U * kF8TileBytes + r_at * 16, p.ws + u_at * U4 * 128 + r_at * 4, p.U);
+      const float sc = o.score != nullptr && sorted ? o.score[row] : 1.f;
+      const float t = fmaxf(fmaxf(s_top[0][lrow], s_top[1][lrow]), fmaxf(s_top[2][lrow], s_top[3][lrow]));
+      const uint32_t pair = f32_to_bf16_pair(f8_unit(act, v.x * sc, v.y * sc), 0.f), c = (pair & 0x7f80u) == 0x7f80u ? kF8Nan : f8_codes4(pair, 0u, f8_scale_value(f8_scale_of(__float_as_uint(t))));
+      if (lane == 0) smem[lrow * 128 + ((column >> 4) ^ (lrow & 7)) * 16 + (column & 15)] = (unsigned char)c;
     }
     __syncthreads();
 #pragma unroll
@@ -369,6 +459,7 @@ __global__ __launch_bounds__(TW* kWave, PAIRED ? 4 : 2) void fp8_tiles_kernel(F8
   __shared__ __attribute__((aligned(1024))) unsigned char smem[Ring<PAIRED>::kLds];
   __shared__ float s_top[GATED ? TWC : 1][64 * Ring<PAIRED>::kHighest];
   __shared__ int s_found[3];
+  __shared__ F8Near<GATED ? 64 * Ring<PAIRED>::kHighest : 1> s_near;
   const int lane = threadIdx.x & (kWave - 1);
   const int slot = blockIdx.x;
   const int c0 = slot / (kSideBySide * p.tiles) * kSideBySide, left = slot - c0 * p.tiles, wide = min(kSideBySide, p.nb - c0);
@@ -431,7 +522,7 @@ __global__ __launch_bounds__(TW* kWave, PAIRED ? 4 : 2) void fp8_tiles_kernel(F8
   }
   const int rows = row_end - row0;
   if (rows <= 0) return;
-#define F8_TILE(MTV) f8_tile<MTV, NT, GATED, PAIRED, TO>(p, o, act, e, row0, row_end, nblock, smem, s_top)
+#define F8_TILE(MTV) f8_tile<MTV, NT, GATED, PAIRED, TO>(p, o, act, e, row0, row_end, nblock, smem, s_top, reinterpret_cast<F8Near<64 * Ring<PAIRED>::kHighest>*>(&s_near))
   if (rows <= 64) F8_TILE(1);
   else if (PAIRED || rows <= 128) F8_TILE(2);
   else if constexpr (!PAIRED) {
