@@ -8,9 +8,9 @@
 //
 // Bound: 8,192 x 16,384 x 5,120 takes 540 us, 2.5 PFLOP/s, by power: the matrix cores are busy 74 % of the time at 1.5 GHz, and a loop of that instruction on
 // registers alone runs at 4.8 PFLOP/s.  The library's product in 8 bits (one scale a tensor) reaches 3.0 PFLOP/s at 8,192 x 8,192 x 8,192.
-// Experts of few rows are bound by reading their weights: 16 of 2 x 8,192 x 5,120 with 6 rows each and one always on, 234 us, 6.1 TB/s.  With more rows the products'
+// Experts of few rows are bound by reading their weights: 16 of 2 x 8,192 x 5,120 with 6 rows each and one always on, 249 us, 5.7 TB/s.  With more rows the products'
 // power and the memory's add up: a step of a tile of 16, 64, 128 and 256 rows over 5,120 takes 0.73, 0.88, 1.02 and 1.35 us with weights from memory, of 256 rows
-// with weights in the caches 0.88 (16 experts with 128 rows each 331 us, 4.1 TB/s, at 1.9 GHz).  Blocks that begin at places of k of their own: no change (337).
+// with weights in the caches 0.88 (16 experts with 128 rows each 364 us, 3.7 TB/s, at 1.9 GHz).  Blocks that begin at places of k of their own: no change.
 // Weights straight into registers instead of through LDS: 600 us for the first product above, then at 579.
 #include <type_traits>
 
@@ -55,7 +55,7 @@ __device__ __forceinline__ int row_piece(int row, int piece) { return piece ^ ((
 
 // Two kernels.  PAIRED: tiles of up to 128 rows, two blocks a compute unit, which fill each other's gaps (a tile's first loads, its barriers, its
 // end); the other: tiles of up to 256, one block a unit, for what many rows share.
-// (us, paired and not: 64 experts of 2 x 1,408 x 2,048, 94 rows each 100 and 105; 16 of 16,384 x 5,120, 128 rows each 357 and 331.)
+// (us, paired and not: 64 experts of 2 x 1,408 x 2,048, 94 rows each 108 and 119; 16 of 16,384 x 5,120, 128 rows each 383 and 364.)
 // LDS holds a ring of slots, a slot one step (64 of k: 16 KB of weights, 4 KB of rows for each MT), or two steps of low tiles in a block of its own,
 // whose steps are short beside a barrier.
 constexpr int step_bytes(int mt, int nt) { return 8192 * nt + 4096 * mt; }

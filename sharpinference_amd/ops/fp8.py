@@ -411,8 +411,8 @@ def tile_fp8(M: int, N: int, K: int, gated: bool, units: int) -> Tuple[int, int,
 
 def grouped_tile_fp8(K: int) -> int:
     """Rows of the tiles of a layer's products at most: over a short k in pairs of blocks a unit, which fill each other's gaps at a tile's start and end (us, tiles of
-    128 and of 256: 64 experts of 2 x 1,408 x 2,048, 94 rows each 100 and 105, 188 146 and 150; 128 of 2 x 768 x 2,048, 125 rows 125 and 132; 16 of 16,384 x 5,120, 38 rows
-    262 and 241, 128 357 and 331; 32 of 5,760 x 2,880, 38 rows 125 and 112, 375 326 and 301).  Of 72 launches timed both ways those it
+    128 and of 256: 64 experts of 2 x 1,408 x 2,048, 94 rows each 108 and 119, 188 159 and 167; 128 of 2 x 768 x 2,048, 125 rows 137 and 146; 16 of 16,384 x 5,120, 38 rows
+    276 and 260, 128 383 and 364; 32 of 5,760 x 2,880, 38 rows 128 and 120, 375 362 and 347).  Of 72 launches timed both ways those it
     chooses take 1.7 % more than the faster ones in the mean (always 256: 3.7 %)."""
     return 128 if K <= 2048 else 256
 
