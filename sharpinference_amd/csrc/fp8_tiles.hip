@@ -4,7 +4,7 @@
 //   gated   act(s g) (s u) with (g | u) the product, rounded to bfloat16 and quantised again: codes and scale bytes of the rows that the
 //           second half of a feed-forward reads.  A block's 128 output columns are one block of the format, so the epilogue has what
 //           it needs, and neither (g | u) nor the unquantised rows go to memory.
-// Every output is one chain over k in ascending order (of each share of it): a row's result does not depend on which rows share its tile.
+// Every output is one chain over k in ascending order (of each share of it): a row's result does not depend on which rows share its tile (but see F8Near::kMost).
 //
 // Bound: 8,192 x 16,384 x 5,120 takes 540 us, 2.5 PFLOP/s, by power: the matrix cores are busy 74 % of the time at 1.5 GHz, and a loop of that instruction on
 // registers alone runs at 4.8 PFLOP/s.  The library's product in 8 bits (one scale a tensor) reaches 3.0 PFLOP/s at 8,192 x 8,192 x 8,192.
@@ -74,12 +74,12 @@ template <bool PAIRED> struct Ring {
 // bfloat16.  Values h that kNear |h| / top of them would move, if they are at least 1 / kNearTop of their block's largest, top (they carry most of the
 // error), are computed once more in float from their rows of codes: about 5 of a tile of 256 x 128, in 4 to 8 us of a tile's 30 to 80 (3,001 rows through
 // 2 x 2,816 x 2,048 53 -> 64 us, 2,048 through 16 experts of 2 x 8,192 x 5,120 and one always on 473 -> 525).  Over 1,700 sizes the layer's error against 64 bits is
-// 1.11 times that of the same sums in float (1.36 at most), without this 1.34 (3.6).  A tile with more than kMost of them (values on borders all
-// along) is left as it is.  The whole product on the bfloat16 instruction would take twice the matrix cores' time.
+// 1.11 times that of the same sums in float (1.36 at most), without this 1.34 (3.6).  A tile with more than kMost of them (the same row again and
+// again, or values on borders all along) is left as it is.  The whole product on the bfloat16 instruction would take twice the matrix cores' time.
 constexpr float kNear = 1.5e-4f;
 constexpr float kNearTop = 4.f;
-template <int ROWS> struct F8Near {
-  static constexpr int kMost = 2 * ROWS;
+struct F8Near {
+  static constexpr int kMost = 128;
   int total;
   unsigned short list[kMost];                  // row of the tile << 7 | column
 };
@@ -131,7 +131,7 @@ template <int kFlight> __device__ __forceinline__ float2 f8_row_dots(const uint8
 // One tile: rows row0 .. row_end (up to 64 MT of them) of matrix e against column block nblock.  MT: groups of 32 rows a wave; NT: weight tiles of a wave.
 template <int MT, int NT, bool GATED, bool PAIRED, typename TO>
 __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedAct act, int e, int row0, int row_end, int nblock, unsigned char* smem,
-                                        float (*s_top)[64 * Ring<PAIRED>::kHighest], F8Near<64 * Ring<PAIRED>::kHighest>* near) {
+                                        float (*s_top)[64 * Ring<PAIRED>::kHighest], F8Near* near) {
   using RG = Ring<PAIRED>;
   constexpr int NS = RG::steps(MT), RING = RG::slots(MT) * NS, AHEAD = RING - NS;      // (steps)
   static_assert(NT == 2 || !GATED, "a gated tile's columns are a block of the format");
@@ -459,7 +459,7 @@ __global__ __launch_bounds__(TW* kWave, PAIRED ? 4 : 2) void fp8_tiles_kernel(F8
   __shared__ __attribute__((aligned(1024))) unsigned char smem[Ring<PAIRED>::kLds];
   __shared__ float s_top[GATED ? TWC : 1][64 * Ring<PAIRED>::kHighest];
   __shared__ int s_found[3];
-  __shared__ F8Near<GATED ? 64 * Ring<PAIRED>::kHighest : 1> s_near;
+  __shared__ F8Near s_near;
   const int lane = threadIdx.x & (kWave - 1);
   const int slot = blockIdx.x;
   const int c0 = slot / (kSideBySide * p.tiles) * kSideBySide, left = slot - c0 * p.tiles, wide = min(kSideBySide, p.nb - c0);
@@ -522,7 +522,7 @@ __global__ __launch_bounds__(TW* kWave, PAIRED ? 4 : 2) void fp8_tiles_kernel(F8
   }
   const int rows = row_end - row0;
   if (rows <= 0) return;
-#define F8_TILE(MTV) f8_tile<MTV, NT, GATED, PAIRED, TO>(p, o, act, e, row0, row_end, nblock, smem, s_top, reinterpret_cast<F8Near<64 * Ring<PAIRED>::kHighest>*>(&s_near))
+#define F8_TILE(MTV) f8_tile<MTV, NT, GATED, PAIRED, TO>(p, o, act, e, row0, row_end, nblock, smem, s_top, &s_near)
   if (rows <= 64) F8_TILE(1);
   else if (PAIRED || rows <= 128) F8_TILE(2);
   else if constexpr (!PAIRED) {

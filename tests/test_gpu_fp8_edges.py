@@ -75,6 +75,21 @@ def test_many_tokens_some_without_an_expert(T, k):
     _close(ops.experts_fp8(x, ids, wts, p1, p2), *_layer_want(x, ids, wts, w1, w2, "silu", False, False))
 
 
+@pytest.mark.parametrize("M,K,I", [(70, 128, 128), (300, 512, 700), (1000, 256, 2100)])
+def test_one_row_again_and_again(M, K, I):
+    """A value near a border of two codes is so in every row: a tile may hold hundreds."""
+    from sharpinference_amd import ops
+    g = _gen(M, K, I)
+    x = _whole(g, 1, K).bfloat16().expand(M, K).contiguous()
+    w1, w2 = _whole(g, 2 * I, K) / 64, _normal(g, 40, I)
+    p1, p2 = ops.quantize_weight(w1, True), ops.quantize_weight(w2)
+    y = ops.feed_forward_fp8(x, p1, p2)
+    want, bound = plain.feed_forward(x[:1].double(), w1.double(), plain.rows(w2), "silu")
+    assert ((y.double() - want).abs() <= bound + plain.stored(want)).all()
+    for _ in range(3):
+        assert torch.equal(ops.feed_forward_fp8(x, p1, p2), y)
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu_tanh", ("swish_clamp", 7.0)])
 @pytest.mark.parametrize("height,M,K,I", [(256, 2048, 640, 2048), (128, 1000, 384, 4096), (192, 1537, 1100, 1500)])
 def test_large_gated_values_near_a_border_have_the_definitions_codes(height, M, K, I, act):
