@@ -4,7 +4,7 @@
 //   gated   act(s g) (s u) with (g | u) the product, rounded to bfloat16 and quantised again: codes and scale bytes of the rows that the
 //           second half of a feed-forward reads.  A block's 128 output columns are one block of the format, so the epilogue has what
 //           it needs, and neither (g | u) nor the unquantised rows go to memory.
-// Every output is one chain over k in ascending order (of each share of it): a row's result does not depend on which rows share its tile (but see F8Near::kMost).
+// Every output is one chain over k in ascending order (of each share of it): a row's result does not depend on which rows share its tile.
 //
 // Bound: 8,192 x 16,384 x 5,120 takes 540 us, 2.5 PFLOP/s, by power: the matrix cores are busy 74 % of the time at 1.5 GHz, and a loop of that instruction on
 // registers alone runs at 4.8 PFLOP/s.  The library's product in 8 bits (one scale a tensor) reaches 3.0 PFLOP/s at 8,192 x 8,192 x 8,192.
@@ -74,15 +74,10 @@ template <bool PAIRED> struct Ring {
 // bfloat16.  Values h that kNear |h| / top of them would move, if they are at least 1 / kNearTop of their block's largest, top (they carry most of the
 // error), are computed once more in float from their rows of codes: about 5 of a tile of 256 x 128, in 4 to 8 us of a tile's 30 to 80 (3,001 rows through
 // 2 x 2,816 x 2,048 53 -> 64 us, 2,048 through 16 experts of 2 x 8,192 x 5,120 and one always on 473 -> 525).  Over 1,700 sizes the layer's error against 64 bits is
-// 1.11 times that of the same sums in float (1.36 at most), without this 1.34 (3.6).  A tile with more than kMost of them (the same row again and
-// again, or values on borders all along) is left as it is.  The whole product on the bfloat16 instruction would take twice the matrix cores' time.
+// 1.11 times that of the same sums in float (1.36 at most), without this 1.34 (3.6).  The list has room for all of a tile's values, behind its codes in the ring: a row's
+// codes are the same alone, again and again in one tile, and beside any others.  The whole product on the bfloat16 instruction would take twice the matrix cores' time.
 constexpr float kNear = 1.5e-4f;
 constexpr float kNearTop = 4.f;
-struct F8Near {
-  static constexpr int kMost = 128;
-  int total;
-  unsigned short list[kMost];                  // row of the tile << 7 | column
-};
 // Two columns' products of a row in float, dealt to the wave: x: the row's codes and scales; w: a column's first piece in its tile, ws: its scales.
 // kFlight: pieces of a lane on their way at a time.
 template <int kFlight> __device__ __forceinline__ float2 f8_row_dots(const uint8_t* __restrict__ x, const uint8_t* __restrict__ xs, const uint8_t* __restrict__ w0, const uint8_t* __restrict__ ws0,
@@ -131,7 +126,7 @@ template <int kFlight> __device__ __forceinline__ float2 f8_row_dots(const uint8
 // One tile: rows row0 .. row_end (up to 64 MT of them) of matrix e against column block nblock.  MT: groups of 32 rows a wave; NT: weight tiles of a wave.
 template <int MT, int NT, bool GATED, bool PAIRED, typename TO>
 __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedAct act, int e, int row0, int row_end, int nblock, unsigned char* smem,
-                                        float (*s_top)[64 * Ring<PAIRED>::kHighest], F8Near* near) {
+                                        float (*s_top)[64 * Ring<PAIRED>::kHighest], int* n_near) {
   using RG = Ring<PAIRED>;
   constexpr int NS = RG::steps(MT), RING = RG::slots(MT) * NS, AHEAD = RING - NS;      // (steps)
   static_assert(NT == 2 || !GATED, "a gated tile's columns are a block of the format");
@@ -372,6 +367,9 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
     const int U2 = f8_blocks(o.n_out), su2 = f8_scale_stride(o.n_out);
     float h[MT][16];
     bool bad = false;                              // (a value of the lane's is not finite)
+    // the values near a border, each row << 7 | column of the tile, behind the codes
+    static_assert(64 * MT * kF8Block * 3 <= RG::slots(MT) * NS * kStep, "codes and a list of all of them fit in the ring");
+    unsigned short* near = reinterpret_cast<unsigned short*>(smem + 64 * MT * kF8Block);
     auto units = [&](auto code_tag) {              // (the activation is chosen once a tile)
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
@@ -394,7 +392,7 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
     if (act.code == ACT_SWISH_CLAMP) units(std::integral_constant<int, ACT_SWISH_CLAMP>{});
     else if (act.code == ACT_GELU_TANH) units(std::integral_constant<int, ACT_GELU_TANH>{});
     else units(std::integral_constant<int, ACT_SILU>{});
-    if (threadIdx.x == 0) near->total = 0;
+    if (threadIdx.x == 0) *n_near = 0;
     __syncthreads();
     // the codes through LDS, to leave as whole lines: a row's 128 are one block of the format
 #pragma unroll
@@ -414,10 +412,8 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
           c = codes_of(0.f);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (const float a = fabsf(h[m][4 * q + i]); (differ >> (8 * i) & 0xff) && a * kNearTop >= t && a <= t * 1.01f && row0 + lrow < row_end) {
-              const int n = atomicAdd(&near->total, 1);
-              if (n < near->kMost) near->list[n] = (unsigned short)(lrow << 7 | (wc * 32 + q * 8 + g * 4 + i));
-            }
+            if (const float a = fabsf(h[m][4 * q + i]); (differ >> (8 * i) & 0xff) && a * kNearTop >= t && a <= t * 1.01f && row0 + lrow < row_end)
+              near[atomicAdd(n_near, 1)] = (unsigned short)(lrow << 7 | (wc * 32 + q * 8 + g * 4 + i));
         }
         if (bad)
 #pragma unroll
@@ -428,9 +424,9 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
       if (wc == 0 && g == 0 && row0 + lrow < row_end) o.scales[(size_t)(row0 + lrow) * su2 + nblock] = (uint8_t)s;
     }
     __syncthreads();
-    const int total = __builtin_amdgcn_readfirstlane(near->total);
-    for (int i = wid; i < total && total <= near->kMost; i += TW) {
-      const int entry = __builtin_amdgcn_readfirstlane(near->list[i]), lrow = entry >> 7, column = entry & 127, row = row0 + lrow, r_at = column & 31;
+    const int total = __builtin_amdgcn_readfirstlane(*n_near);
+    for (int i = wid; i < total; i += TW) {
+      const int entry = __builtin_amdgcn_readfirstlane(near[i]), lrow = entry >> 7, column = entry & 127, row = row0 + lrow, r_at = column & 31;
       const size_t x_at = x_first + __builtin_amdgcn_readfirstlane(x_row(lrow));
       const size_t g_at = w_at + block_tile(2 * (column >> 5)), u_at = w_at + block_tile(2 * (column >> 5) + 1);
       const float2 v = f8_row_dots<PAIRED ? 3 : 6>(p.x + x_at * x_stride, p.xs + x_at * (U4 * 4), p.w + g_at * p.U * kF8TileBytes + r_at * 16, p.ws + g_at * U4 * 128 + r_at * 4,
@@ -459,7 +455,7 @@ __global__ __launch_bounds__(TW* kWave, PAIRED ? 4 : 2) void fp8_tiles_kernel(F8
   __shared__ __attribute__((aligned(1024))) unsigned char smem[Ring<PAIRED>::kLds];
   __shared__ float s_top[GATED ? TWC : 1][64 * Ring<PAIRED>::kHighest];
   __shared__ int s_found[3];
-  __shared__ F8Near s_near;
+  __shared__ int s_near;
   const int lane = threadIdx.x & (kWave - 1);
   const int slot = blockIdx.x;
   const int c0 = slot / (kSideBySide * p.tiles) * kSideBySide, left = slot - c0 * p.tiles, wide = min(kSideBySide, p.nb - c0);
