@@ -29,7 +29,7 @@ constexpr int kF8Block = 128;                 // values that share a scale
 constexpr int kF8Tile = 32;                   // weight rows of a tile
 constexpr int kF8TileBytes = kF8Tile * kF8Block;
 constexpr uint32_t kF8Nan = 0x7f;
-constexpr int kF8MostK = 1 << 24;             // columns of a row at most: 256 rows of codes are 2^32 bytes, what a tile's loads reach
+constexpr int kF8MostK = 1 << 24;             // columns of a row at most.  (A tile's loads reach 2^32 - 1 bytes of codes: 256 rows of up to 2^24 - 128, 192 of all)
 
 static inline __host__ __device__ int f8_blocks(int k) { return (k + kF8Block - 1) / kF8Block; }
 static inline __host__ __device__ int f8_scale_stride(int k) { return (f8_blocks(k) + 3) & ~3; }     // bytes of a row's scales

@@ -538,6 +538,7 @@ bool tiles_ok(const F8Tiles& p, int x_rows) {
 template <bool GATED> int launch_tiles(F8Tiles p, const F8Out& o, GatedAct act, int nt, int dtype, hipStream_t stream) {
   const int height = p.height;
   if (height < 64 || height > 64 * Ring<false>::kHighest || height % 64) return SHARPI_ERR_ARG;
+  if (!p.a_rows && (long long)height * p.U * kF8Block > 0xffffffffLL) return SHARPI_ERR_ARG;      // (a tile's rows: one descriptor of its loads)
   const long long tiles = p.offsets ? (long long)p.rows / height + (p.rows < p.groups ? p.rows : p.groups) + (p.along + height - 1) / height
                                     : (p.rows + height - 1) / height;
   if ((nt != 1 && nt != 2) || (nt == 1 && (GATED || height <= 64 * Ring<true>::kHighest))) return SHARPI_ERR_ARG;

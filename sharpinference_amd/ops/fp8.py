@@ -27,6 +27,7 @@ FP8_FEW_PAIRS = 512            # (token, pick) pairs of the same (kFewPairs)
 FP8_LAYER_COLUMNS = 32         # columns of the sum that a block takes (16 kLayerTiles)
 FP8_MAX_EXPERTS = 1023         # experts of a layer, one more may be always on (kFewExperts, kMaxGroups)
 FP8_MOST_K = (1 << 24) - 1     # columns of a row (kF8MostK)
+FP8_TILE_REACH = (1 << 32) - 1 # bytes of codes that the loads of a tile's rows reach
 # rows of bfloat16 that the weight-streaming kernels quantise where they read them, in every block, instead of in a launch ahead (us of a layer's launches, staged
 # and ahead: an expert of 16 of 5,120 x 8,192 and one always on, 1 token 54.6 and 55.8, 2 73.0 and 76.3, 4 108.7 and 103.6, 8 164 and 142; six of 64 of 2,048 x 1,408, 1 token
 # 26.0 and 28.1, 2 35.9 and 38.6, 4 51.7 and 49.5)
@@ -388,6 +389,11 @@ TILE_END_US = 5.0
 JOIN_US, JOIN_TBS = 3.0, 6.0      # adding shares up: a launch, and the rate at which they are written and read again
 
 
+def _highest(K: int) -> int:
+    """Rows of a tile at most, which its loads have to reach: 256, or 192 of the widest."""
+    return min(256, FP8_TILE_REACH // (_blocks(K) * FP8_BLOCK) // 64 * 64)
+
+
 @functools.lru_cache(maxsize=1024)
 def tile_fp8(M: int, N: int, K: int, gated: bool, units: int) -> Tuple[int, int, int]:
     """(rows, columns / 128, shares of k) of the tiles of a product of many rows (gated: 256 columns, one share): those whose rounds of the chip take the
@@ -406,7 +412,7 @@ def tile_fp8(M: int, N: int, K: int, gated: bool, units: int) -> Tuple[int, int,
         return us + (JOIN_US + 8e-6 * shares * M * N / JOIN_TBS if shares > 1 else 0.0)
     choices = [(64, 2), (128, 2), (192, 2), (256, 2)] + ([] if gated else [(192, 1), (256, 1)])
     most = 1 if gated else min(8, max(1, _blocks(K) // 4))
-    return min(((h, nt, s) for h, nt in choices for s in range(1, most + 1)), key=lambda c: expected(*c))
+    return min(((h, nt, s) for h, nt in choices if h <= _highest(K) for s in range(1, most + 1)), key=lambda c: expected(*c))
 
 
 def grouped_tile_fp8(K: int) -> int:
@@ -414,7 +420,7 @@ def grouped_tile_fp8(K: int) -> int:
     128 and of 256: 64 experts of 2 x 1,408 x 2,048, 94 rows each 108 and 119, 188 159 and 167; 128 of 2 x 768 x 2,048, 125 rows 137 and 146; 16 of 16,384 x 5,120, 38 rows
     276 and 260, 128 383 and 364; 32 of 5,760 x 2,880, 38 rows 128 and 120, 375 362 and 347).  Of 72 launches timed both ways those it
     chooses take 1.7 % more than the faster ones in the mean (always 256: 3.7 %)."""
-    return 128 if K <= 2048 else 256
+    return 128 if K <= 2048 else _highest(K)
 
 
 def _layer_checked(x, w_gate_up: Fp8Weight, w_down: Fp8Weight, dims: int, who: str):
