@@ -41,6 +41,9 @@ __device__ __forceinline__ int f8_scale_of(uint32_t top_bits) {
   return s < 1 ? 1 : s;
 }
 __device__ __forceinline__ float f8_scale_value(int s) { return __uint_as_float((uint32_t)s << 23); }
+// A block's sum of products of codes, times the scales of both operands, whose bytes are given added up: one step of the exponent, whatever either scale is
+// by itself.
+__device__ __forceinline__ float f8_scaled(float sum, int bytes) { return __builtin_amdgcn_ldexpf(sum, bytes - 254); }
 
 typedef __attribute__((ext_vector_type(2))) short s16x2_t;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2v_t;

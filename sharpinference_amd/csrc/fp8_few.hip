@@ -52,11 +52,12 @@ struct F8Lane {
     codes = w.codes + tile * w.U * kF8TileBytes + (t & 1) * 256;
     scales = w.scales + tile * ((w.U + 3) >> 2) * 128 + (t & 1) * 64;
   }
-  __device__ __forceinline__ i32x8 load(int u, int r, int g, int& s) const {
+  // a lane's codes of row r, and the scale byte of row scale_row
+  __device__ __forceinline__ i32x8 load(int u, int r, int g, int scale_row, int& s) const {
     const uint8_t* from = codes + (size_t)u * kF8TileBytes + (uint32_t)((g >> 1) * 2048 + (g & 1) * 512 + r * 16);
     const i32x4 a = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(from));
     const i32x4 b = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(from + 1024));
-    s = (scales + (u >> 2) * 128 + (u & 3))[(uint32_t)r * 4];
+    s = (scales + (u >> 2) * 128 + (u & 3))[(uint32_t)scale_row * 4];
     return i32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   }
 };
@@ -140,32 +141,35 @@ __device__ __forceinline__ f32x4 f8_product(const i32x8& w, const i32x8& x, cons
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 0, 0, 0, ws, 0, xs);
 }
 
-// The same with every product and sum in float: codes widened to bfloat16, which holds them, the weights' with their scale; the rows' scale on the block's
-// sum.  For results that are quantised again: what the scaled instruction leaves out moves a value in 2,000 across a border of e4m3, 1 / 16 of
-// it, and the layer's error against 64 bits was 1.5 times that of the same sums in float.  The widening is hidden by the weights' way from memory.
+// The same with every product and sum in float: codes widened to bfloat16, which holds them, and both scales on the block's sum, whose exponent holds
+// them together (a weight's scale times its code may lie beyond bfloat16, and beyond float its product with a row's code).  For results that are
+// quantised again: what the scaled instruction leaves out moves now and then a value across a border of e4m3, 1 / 16 of it, and the layer's error
+// against 64 bits was 1.5 times that of the same sums in float.  The widening is hidden by the weights' way from memory.
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
-__device__ __forceinline__ bf16x8 f8_wide(int lo, int hi, float scale) {
+__device__ __forceinline__ bf16x8 f8_wide(int lo, int hi) {
   typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
-  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)lo, scale, true);
-  const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)hi, scale, true);
+  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)lo, 1.0f, true);
+  const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)hi, 1.0f, true);
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
+// ws: of the four rows whose sums a lane ends up with, g * 4 + 0 .. 3, the four neighbouring lanes hold a scale byte each.
+template <int I> __device__ __forceinline__ int f8_byte_of(int ws) { return __builtin_amdgcn_update_dpp(0, ws, I * 0x55, 0xf, 0xf, true); }
 template <int R> __device__ __forceinline__ void f8_product_in_float(const i32x8 (&w)[R], const int (&ws)[R], const i32x8& x, int xs, f32x4* acc, int step) {
   f32x4 sum[R];
 #pragma unroll
   for (int t = 0; t < R; ++t) sum[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const bf16x8 xw = f8_wide(x[2 * j], x[2 * j + 1], 1.0f);
+    const bf16x8 xw = f8_wide(x[2 * j], x[2 * j + 1]);
 #pragma unroll
-    for (int t = 0; t < R; ++t)
-      sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f8_wide(w[t][2 * j], w[t][2 * j + 1], f8_scale_value(ws[t])), xw, sum[t], 0, 0, 0);
+    for (int t = 0; t < R; ++t) sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f8_wide(w[t][2 * j], w[t][2 * j + 1]), xw, sum[t], 0, 0, 0);
   }
-  const float scale = f8_scale_value(xs);
 #pragma unroll
-  for (int t = 0; t < R; ++t)
+  for (int t = 0; t < R; ++t) {
+    const int b[4] = {f8_byte_of<0>(ws[t]), f8_byte_of<1>(ws[t]), f8_byte_of<2>(ws[t]), f8_byte_of<3>(ws[t])};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[t * step][i] = fmaf(sum[t][i], scale, acc[t * step][i]);
+    for (int i = 0; i < 4; ++i) acc[t * step][i] += f8_scaled(sum[t][i], b[i] + xs);
+  }
 }
 
 // Four neighbouring columns from n on of one row of `columns`.
@@ -287,7 +291,7 @@ __global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_few_kernel(cons
     };
     auto load_unit = [&](int u, Unit& un) {
 #pragma unroll
-      for (int t = 0; t < R; ++t) un.wf[t] = wl[t].load(u, r, g, un.ws[t]);
+      for (int t = 0; t < R; ++t) un.wf[t] = wl[t].load(u, r, g, GATED ? g * 4 + (r & 3) : r, un.ws[t]);
       if constexpr (!STAGED) {
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) un.xf[mb].load(x, x_scales, xr[mb], xsr[mb], u);     // (a row block without rows reads the last row)
@@ -480,7 +484,7 @@ __global__ __launch_bounds__(FW* kWave, MB > 1 ? 2 : 4) void fp8_sum_kernel(cons
     for (int t = 0; t < R; ++t) {
       F8Lane wl;
       wl.at(W, code & 0xffff, n_base / 16 + t);
-      un.wf[t] = wl.load(u, r, g, un.ws[t]);
+      un.wf[t] = wl.load(u, r, g, r, un.ws[t]);
     }
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {

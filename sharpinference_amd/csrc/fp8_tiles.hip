@@ -117,7 +117,7 @@ template <int kFlight> __device__ __forceinline__ float2 f8_row_dots(const uint8
         }
       }
 #pragma unroll
-      for (int t = 0; t < 2; ++t) sum[t] = fmaf(s[t] * f8_scale_value(xb[i]), f8_scale_value(wb[t][i]), sum[t]);
+      for (int t = 0; t < 2; ++t) sum[t] += f8_scaled(s[t], xb[i] + wb[t][i]);
     }
   }
   return make_float2(wave_sum(sum[0]), wave_sum(sum[1]));
