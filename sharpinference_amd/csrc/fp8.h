@@ -65,8 +65,9 @@ __device__ __forceinline__ uint32_t f8_codes4(uint32_t lo, uint32_t hi, float sc
 // from the exponent, where the general exponential and division take some 30 instructions an element.
 template <int ACT> __device__ __forceinline__ float f8_unit(float limit, float g, float u) {
   if constexpr (ACT == ACT_SWISH_CLAMP) {
-    g = fminf(g, limit);
-    u = fminf(fmaxf(u, -limit), limit) + 1.0f;
+    // (by comparisons: a NaN stays one, and with it the row of the result)
+    g = g > limit ? limit : g;
+    u = (u > limit ? limit : u < -limit ? -limit : u) + 1.0f;
   }
   const float z = ACT == ACT_SWISH_CLAMP ? kSwishSlope * g : ACT == ACT_GELU_TANH ? 1.5957691216057308f * (g + 0.044715f * g * g * g) : g;
   return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z)) * u;
