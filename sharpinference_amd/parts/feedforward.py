@@ -71,11 +71,14 @@ class DenseSwiGLU(Part):
                         prefix + n["down"] + self.bias_suffix: ParamSpec((self.hidden,))})
         return out
 
-    def load(self, prefix: str, source: TensorSource) -> None:
+    def load(self, prefix: str, source: TensorSource, in_8_bits: Optional[bool] = None) -> None:
+        """in_8_bits: whether the matrices may be kept in 8 bits (None: as ``ops.feed_forwards_in_8_bits`` says)."""
         n = self.names
         g = source.get(prefix + n["gate"])
         u = source.get(prefix + n["up"])
-        if ops.feed_forwards_are_8_bits() and not self.bias and g.dtype == u.dtype == torch.bfloat16:
+        if in_8_bits is None:
+            in_8_bits = ops.feed_forwards_are_8_bits()
+        if in_8_bits and not self.bias and g.dtype == u.dtype == torch.bfloat16:
             self.w_gate_up = ops.quantize_weight(_fuse_rows(g, u), gated=True)
             del g, u
             self.w_down = ops.quantize_weight(source.get(prefix + n["down"]))
@@ -157,7 +160,8 @@ class MoESwiGLU(Part):
     Their share is added where the outputs are summed (``ops.ExpertSum``).
 
     Loaded under ``ops.feed_forwards_in_8_bits`` gated experts (up to 1,023) without identity experts beside them, of bfloat16 matrices, are kept
-    in 8 bits and run through ``ops.experts_fp8``, a shared expert of their width and activation as one more matrix."""
+    in 8 bits and run through ``ops.experts_fp8``, a shared expert of their width and activation as one more matrix.  Other layers stay
+    as they are, their shared expert included."""
 
     MERGE_MAX_TOKENS = 16   # one row block of the few-rows kernel for the shared group (measured: up to 64 tokens
                             # the merged launches and the library's product for the shared expert are as fast)
@@ -269,13 +273,14 @@ class MoESwiGLU(Part):
         d = self._expert_stack(prefix, "down", source)
         self.merged = False
         sh = self.shared
-        if sh is not None:
-            sh.load(prefix + self.names["shared"], source)
         bf16 = u.dtype == d.dtype == torch.bfloat16 and (g is None or g.dtype == torch.bfloat16)
+        in_8_bits = bf16 and self.gated and not self.identity and self.E <= ops.FP8_MAX_EXPERTS and ops.feed_forwards_are_8_bits()
+        if sh is not None:                                # (a layer's matrices are all of one kind)
+            sh.load(prefix + self.names["shared"], source, **({"in_8_bits": in_8_bits} if self.gated else {}))
         # The experts' matrices are kept only in the order the kernels stream them (no rows: both
         # the few-rows and the many-rows product of the experts read that order), if the sizes allow.
         pack = bf16 and self.inter % 128 == 0 and self.hidden % 128 == 0
-        if bf16 and self.gated and not self.identity and self.E <= ops.FP8_MAX_EXPERTS and ops.feed_forwards_are_8_bits():
+        if in_8_bits:
             self._load_8_bits(g, u, d)
             return
         sh_first = None if sh is None else "w_gate_up" if self.gated else "w_up"       # the shared expert's first matrix
