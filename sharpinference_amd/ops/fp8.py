@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import contextlib
 import functools
+import threading
 from typing import Optional, Tuple, Union
 
 import torch
@@ -239,18 +240,18 @@ def quantize_weight(w: torch.Tensor, gated: bool = False) -> Fp8Weight:
     return out
 
 
-_FEED_FORWARDS = False
+_SWITCH = threading.local()
 
 
 def feed_forwards_in_8_bits(on: bool) -> None:
     """Whether gated feed-forwards, dense and routed, keep bfloat16 matrices in 8 bits (half of the bytes of a decode step's largest reads) and run
-    through ``feed_forward_fp8`` and ``experts_fp8``.  Read when weights are loaded."""
-    global _FEED_FORWARDS
-    _FEED_FORWARDS = bool(on)
+    through ``feed_forward_fp8`` and ``experts_fp8``.  Read when weights are loaded, by the thread that loads them: it holds for the calling thread alone, so that
+    engines loaded side by side have each their own."""
+    _SWITCH.on = bool(on)
 
 
 def feed_forwards_are_8_bits() -> bool:
-    return _FEED_FORWARDS
+    return getattr(_SWITCH, "on", False)
 
 
 def _new_rows(M: int, k: int, device) -> Fp8Rows:
