@@ -78,49 +78,66 @@ template <bool PAIRED> struct Ring {
 // codes are the same alone, again and again in one tile, and beside any others.  The whole product on the bfloat16 instruction would take twice the matrix cores' time.
 constexpr float kNear = 1.5e-4f;
 constexpr float kNearTop = 4.f;
-// Two columns' products of a row in float, dealt to the wave: x: the row's codes and scales; w: a column's first piece in its tile, ws: its scales.
-// kFlight: pieces of a lane on their way at a time.
-template <int kFlight> __device__ __forceinline__ float2 f8_row_dots(const uint8_t* __restrict__ x, const uint8_t* __restrict__ xs, const uint8_t* __restrict__ w0, const uint8_t* __restrict__ ws0,
-                                              const uint8_t* __restrict__ w1, const uint8_t* __restrict__ ws1, int U) {
+// Of more than kNearMany values kNearRows neighbours of the list go together where they are of one column, whose pieces lie in lines of their own and take longer than the rows': equal rows
+// have all of their values near a border in the same columns.
+constexpr int kNearMany = 64, kNearRows = 4;
+// Two columns' products of ROWS rows in float, dealt to the wave: x: a row's codes and scales; w: a column's first piece in its tile, ws: its scales.  A lane's
+// pieces come in their order, whatever ROWS and kFlight (pieces on their way at a time) are, so every row gets the same sum.
+struct F8Source {
+  const uint8_t* codes;
+  const uint8_t* scales;
+};
+template <int kFlight, int ROWS>
+__device__ __forceinline__ void f8_row_dots(const F8Source (&x)[ROWS], const F8Source (&w)[2], int U, float2 (&out)[ROWS]) {
   typedef __attribute__((ext_vector_type(2))) float f32x2;
   const int lane = threadIdx.x & (kWave - 1), pieces = U * 8;
-  float sum[2] = {0.f, 0.f};
+  float sum[ROWS][2];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) sum[r][0] = sum[r][1] = 0.f;
   for (int p0 = lane; p0 < pieces; p0 += kFlight * kWave) {
-    i32x4 xv[kFlight], wv[2][kFlight];
-    int xb[kFlight], wb[2][kFlight];
+    i32x4 xv[ROWS][kFlight], wv[2][kFlight];
+    int xb[ROWS][kFlight], wb[2][kFlight];
 #pragma unroll
     for (int i = 0; i < kFlight; ++i) {
       const int q = min(p0 + i * kWave, pieces - 1), u = q >> 3, j = q & 7;       // piece j of a block: k = 16 j
       const size_t at = (size_t)u * kF8TileBytes + (j >> 2) * 2048 + (j & 1) * 1024 + (j >> 1 & 1) * 512;
       const int byte = (u >> 2) * 128 + (u & 3);
-      xv[i] = *reinterpret_cast<const i32x4*>(x + (size_t)q * 16);
-      wv[0][i] = *reinterpret_cast<const i32x4*>(w0 + at);
-      wv[1][i] = *reinterpret_cast<const i32x4*>(w1 + at);
-      xb[i] = xs[u];
-      wb[0][i] = ws0[byte];
-      wb[1][i] = ws1[byte];
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        xv[r][i] = *reinterpret_cast<const i32x4*>(x[r].codes + (size_t)q * 16);
+        xb[r][i] = x[r].scales[u];
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        wv[t][i] = *reinterpret_cast<const i32x4*>(w[t].codes + at);
+        wb[t][i] = w[t].scales[byte];
+      }
     }
 #pragma unroll
     for (int i = 0; i < kFlight; ++i) {
       if (p0 + i * kWave >= pieces) continue;
-      float s[2] = {0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(xv[i][c], false), b = __builtin_amdgcn_cvt_pk_f32_fp8(xv[i][c], true);
+      for (int r = 0; r < ROWS; ++r) {
+        float s[2] = {0.f, 0.f};
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const f32x2 d = __builtin_amdgcn_cvt_pk_f32_fp8(wv[t][i][c], false), f = __builtin_amdgcn_cvt_pk_f32_fp8(wv[t][i][c], true);
-          s[t] = fmaf(a[0], d[0], s[t]);
-          s[t] = fmaf(a[1], d[1], s[t]);
-          s[t] = fmaf(b[0], f[0], s[t]);
-          s[t] = fmaf(b[1], f[1], s[t]);
+        for (int c = 0; c < 4; ++c) {
+          const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(xv[r][i][c], false), b = __builtin_amdgcn_cvt_pk_f32_fp8(xv[r][i][c], true);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const f32x2 d = __builtin_amdgcn_cvt_pk_f32_fp8(wv[t][i][c], false), f = __builtin_amdgcn_cvt_pk_f32_fp8(wv[t][i][c], true);
+            s[t] = fmaf(a[0], d[0], s[t]);
+            s[t] = fmaf(a[1], d[1], s[t]);
+            s[t] = fmaf(b[0], f[0], s[t]);
+            s[t] = fmaf(b[1], f[1], s[t]);
+          }
         }
-      }
 #pragma unroll
-      for (int t = 0; t < 2; ++t) sum[t] += f8_scaled(s[t], xb[i] + wb[t][i]);
+        for (int t = 0; t < 2; ++t) sum[r][t] += f8_scaled(s[t], xb[r][i] + wb[t][i]);
+      }
     }
   }
-  return make_float2(wave_sum(sum[0]), wave_sum(sum[1]));
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) out[r] = make_float2(wave_sum(sum[r][0]), wave_sum(sum[r][1]));
 }
 
 // One tile: rows row0 .. row_end (up to 64 MT of them) of matrix e against column block nblock.  MT: groups of 32 rows a wave; NT: weight tiles of a wave.
@@ -425,16 +442,55 @@ __device__ __forceinline__ void f8_tile(const F8Tiles& p, const F8Out& o, GatedA
     }
     __syncthreads();
     const int total = __builtin_amdgcn_readfirstlane(*n_near);
-    for (int i = wid; i < total; i += TW) {
-      const int entry = __builtin_amdgcn_readfirstlane(near[i]), lrow = entry >> 7, column = entry & 127, row = row0 + lrow, r_at = column & 31;
-      const size_t x_at = x_first + __builtin_amdgcn_readfirstlane(x_row(lrow));
-      const size_t g_at = w_at + block_tile(2 * (column >> 5)), u_at = w_at + block_tile(2 * (column >> 5) + 1);
-      const float2 v = f8_row_dots<PAIRED ? 3 : 6>(p.x + x_at * x_stride, p.xs + x_at * (U4 * 4), p.w + g_at * p.U * kF8TileBytes + r_at * 16, p.ws + g_at * U4 * 128 + r_at * 4,
-                                                   p.w + u_at * p.U * kF8TileBytes + r_at * 16, p.ws + u_at * U4 * 128 + r_at * 4, p.U);
-      const float sc = o.score != nullptr && sorted ? o.score[row] : 1.f;
-      const float t = fmaxf(fmaxf(s_top[0][lrow], s_top[1][lrow]), fmaxf(s_top[2][lrow], s_top[3][lrow]));
-      const uint32_t pair = f32_to_bf16_pair(f8_unit(act, v.x * sc, v.y * sc), 0.f), c = (pair & 0x7f80u) == 0x7f80u ? kF8Nan : f8_codes4(pair, 0u, f8_scale_value(f8_scale_of(__float_as_uint(t))));
-      if (lane == 0) smem[lrow * 128 + ((column >> 4) ^ (lrow & 7)) * 16 + (column & 15)] = (unsigned char)c;
+    // values of one column, computed again and put in their places
+    auto again = [&](auto flight_tag, auto rows_tag, const int (&lrow)[decltype(rows_tag)::value], int column) {
+      constexpr int N = decltype(rows_tag)::value;
+      auto source = [&](int which) {
+        const size_t at = w_at + block_tile(2 * (column >> 5) + which);
+        return F8Source{p.w + at * p.U * kF8TileBytes + (column & 31) * 16, p.ws + at * U4 * 128 + (column & 31) * 4};
+      };
+      const F8Source w[2] = {source(0), source(1)};
+      F8Source x[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const size_t x_at = x_first + __builtin_amdgcn_readfirstlane(x_row(lrow[j]));
+        x[j] = {p.x + x_at * x_stride, p.xs + x_at * (U4 * 4)};
+      }
+      float2 v[N];
+      f8_row_dots<decltype(flight_tag)::value, N>(x, w, p.U, v);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float sc = o.score != nullptr && sorted ? o.score[row0 + lrow[j]] : 1.f;
+        const float t = fmaxf(fmaxf(s_top[0][lrow[j]], s_top[1][lrow[j]]), fmaxf(s_top[2][lrow[j]], s_top[3][lrow[j]]));
+        const uint32_t pair = f32_to_bf16_pair(f8_unit(act, v[j].x * sc, v[j].y * sc), 0.f);
+        const uint32_t c = (pair & 0x7f80u) == 0x7f80u ? kF8Nan : f8_codes4(pair, 0u, f8_scale_value(f8_scale_of(__float_as_uint(t))));
+        if (lane == 0) smem[lrow[j] * 128 + ((column >> 4) ^ (lrow[j] & 7)) * 16 + (column & 15)] = (unsigned char)c;
+      }
+    };
+    const bool many = total > kNearMany;
+    for (int i = many ? wid * kNearRows : wid; i < total; i += many ? TW * kNearRows : TW) {
+      int left = 1;
+      if (many) {
+        left = min(kNearRows, total - i);
+        int lrow[kNearRows];
+        const int column = __builtin_amdgcn_readfirstlane(near[i]) & 127;
+        bool same = left == kNearRows;
+#pragma unroll
+        for (int j = 0; j < kNearRows; ++j) {
+          const int entry = __builtin_amdgcn_readfirstlane(near[min(i + j, total - 1)]);
+          lrow[j] = entry >> 7;
+          same = same && (entry & 127) == column;
+        }
+        if (same) {
+          again(std::integral_constant<int, 1>{}, std::integral_constant<int, kNearRows>{}, lrow, column);
+          left = 0;
+        }
+      }
+#pragma unroll 1
+      for (int j = 0; j < left; ++j) {
+        const int entry = __builtin_amdgcn_readfirstlane(near[i + j]), one[1] = {entry >> 7};
+        again(std::integral_constant<int, PAIRED ? 3 : 6>{}, std::integral_constant<int, 1>{}, one, entry & 127);
+      }
     }
     __syncthreads();
 #pragma unroll
