@@ -6,11 +6,12 @@
 //           it needs, and neither (g | u) nor the unquantised rows go to memory.
 // Every output is one chain over k in ascending order (of each share of it): a row's result does not depend on which rows share its tile.
 //
-// Bound: 8,192 x 16,384 x 5,120 takes 540 us, 2.5 PFLOP/s, by power: the matrix cores are busy 74 % of the time at 1.5 GHz, and a loop of that instruction on
-// registers alone runs at 4.8 PFLOP/s.  The library's product in 8 bits (one scale a tensor) reaches 3.0 PFLOP/s at 8,192 x 8,192 x 8,192.
+// Bound: 8,192 x 16,384 x 5,120 takes 547 us at best, 2.5 PFLOP/s, and 597 in a run of many (2.3): power takes the clock from 2.4 down to 1.5 to 1.7 GHz, of which the matrix
+// cores are busy 73 %.  A loop of that instruction on registers alone runs at 4.8 PFLOP/s; the library's product in 8 bits (one scale a tensor) at 3.0 at 8,192 x 8,192 x
+// 8,192, busy 90 % at 1.70 GHz, where these tiles are busy 77 % at 1.50: what is left to gain are waits, and power spent beside the products.
 // Experts of few rows are bound by reading their weights: 16 of 2 x 8,192 x 5,120 with 6 rows each and one always on, 249 us, 5.7 TB/s.  With more rows the products'
 // power and the memory's add up: a step of a tile of 16, 64, 128 and 256 rows over 5,120 takes 0.73, 0.88, 1.02 and 1.35 us with weights from memory, of 256 rows
-// with weights in the caches 0.88 (16 experts with 128 rows each 364 us, 3.7 TB/s, at 1.9 GHz).  Blocks that begin at places of k of their own: no change.
+// with weights in the caches 0.88 (16 experts with 128 rows each 364 us, 3.7 TB/s; the clock is at 2.0 GHz, the matrix cores busy 38 %).  Blocks that begin at places of k of their own: no change.
 // Weights straight into registers instead of through LDS: 600 us for the first product above, then at 579.
 #include <type_traits>
 
@@ -55,6 +56,7 @@ __device__ __forceinline__ int row_piece(int row, int piece) { return piece ^ ((
 
 // Two kernels.  PAIRED: tiles of up to 128 rows, two blocks a compute unit, which fill each other's gaps (a tile's first loads, its barriers, its
 // end); the other: tiles of up to 256, one block a unit, for what many rows share.
+// The paired kernels spill up to four vector registers, the gated tall one scalar ones only.
 // (us, paired and not: 64 experts of 2 x 1,408 x 2,048, 94 rows each 108 and 119; 16 of 16,384 x 5,120, 128 rows each 383 and 364.)
 // LDS holds a ring of slots, a slot one step (64 of k: 16 KB of weights, 4 KB of rows for each MT), or two steps of low tiles in a block of its own,
 // whose steps are short beside a barrier.
@@ -70,16 +72,17 @@ template <bool PAIRED> struct Ring {
 };
 
 // Gated results near a border of two codes.  The instruction's products are off by some 2e-5 of a sum's rms (fp8.h), now and then by ten times that, which moves 1
-// value in 500 across a border of e4m3, a sixteenth to an eighth of it: nearly as much error in the layer's result as that result's rounding to
-// bfloat16.  Values h that kNear |h| / top of them would move, if they are at least 1 / kNearTop of their block's largest, top (they carry most of the
+// value in 390 across a border of e4m3 (float sums 1 in 170,000 and fewer), a sixteenth to an eighth of it: nearly as much error in the layer's result as that result's
+// rounding to bfloat16.  Values h that kNear |h| / top of them would move, if they are at least 1 / kNearTop of their block's largest, top (they carry most of the
 // error), are computed once more in float from their rows of codes: about 5 of a tile of 256 x 128, in 4 to 8 us of a tile's 30 to 80 (3,001 rows through
-// 2 x 2,816 x 2,048 53 -> 64 us, 2,048 through 16 experts of 2 x 8,192 x 5,120 and one always on 473 -> 525).  Over 1,700 sizes the layer's error against 64 bits is
-// 1.11 times that of the same sums in float (1.36 at most), without this 1.34 (3.6).  The list has room for all of a tile's values, behind its codes in the ring: a row's
+// 2 x 2,816 x 2,048 57 -> 65 us, 2,048 through 16 experts of 2 x 8,192 x 5,120 and one always on 522 -> 585).  Of these large values 1 in 24,000 or fewer is then off, for 1 in 3,000.  Over
+// 1,400 drawn sizes the layer's error against 64 bits is 1.11 times that of the same sums in float (1.40 at most), without this 1.34 (3.6).  The list has room for all of a tile's values, behind its codes in the ring: a row's
 // codes are the same alone, again and again in one tile, and beside any others.  The whole product on the bfloat16 instruction would take twice the matrix cores' time.
 constexpr float kNear = 1.5e-4f;
 constexpr float kNearTop = 4.f;
 // Of more than kNearMany values kNearRows neighbours of the list go together where they are of one column, whose pieces lie in lines of their own and take longer than the rows': equal rows
-// have all of their values near a border in the same columns.
+// have all of their values near a border in the same columns.  (2,048 equal rows through 2 x 8,192 x 5,120 and back, in the order of their values near a border: 315 to 420 us, by one at a
+// time 412 to 554, where rows that differ take 265; 3,001 through 2 x 2,816 x 2,048 81 to 108, 80 to 142 and 95.)
 constexpr int kNearMany = 64, kNearRows = 4;
 // Two columns' products of ROWS rows in float, dealt to the wave: x: a row's codes and scales; w: a column's first piece in its tile, ws: its scales.  A lane's
 // pieces come in their order, whatever ROWS and kFlight (pieces on their way at a time) are, so every row gets the same sum.
